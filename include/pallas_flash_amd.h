@@ -376,6 +376,90 @@ typedef struct {
 int pf_paged_cache_write(const pf_paged_cache_write_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Rotary positions with several axes (time, height, width of images and
+ * video). No counterpart in the reference, whose tables are indexed by the row
+ * (fused_rope.py:43-50; model.py:41-67). Pair i of a row (elements i and
+ * i + head_dim/2) belongs to axis a where the first sections[0] pairs are axis
+ * 0's, the next sections[1] axis 1's, ...; with p = positions[a][b][s] it is
+ * rotated by table row p as pf_rope rotates by row s (inverse = 1: the
+ * transpose, i.e. the VJP). One axis is RoPE at arbitrary positions. float32
+ * arithmetic, one rounding to dtype.
+ *   q [batch, num_heads, seq_len, head_dim], k the same with num_kv_heads:
+ *     any strides (in elements) of the first three dimensions, the last one
+ *     dense; k may be NULL (num_kv_heads 0: q alone)
+ *   q_out, k_out: dense; may be q, k themselves where those are dense
+ *   positions [axes, batch, seq_len] device int32, or int64 (positions_i64 = 1),
+ *     by positions_stride (elements; 0 = shared). A token with a position
+ *     outside [0, rope_len) on any axis gives zeros.
+ *   cos, sin [rope_len, head_dim] float32
+ *   axes in [1, 4]; sections positive, head_dim / 2 in all
+ *   head_dim: even, any
+ * ------------------------------------------------------------------------- */
+#define PF_MAX_ROPE_AXES 4
+typedef struct {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_stride[3], k_stride[3]; /* batch, head, sequence */
+  const void* positions;
+  int64_t positions_stride[3]; /* axis, batch, sequence */
+  int32_t positions_i64;
+  int32_t axes;
+  int32_t sections[PF_MAX_ROPE_AXES];
+  const float* cos;
+  const float* sin;
+  int32_t rope_len;
+  int32_t batch, num_heads, num_kv_heads, seq_len, head_dim;
+  int32_t inverse;
+  int32_t dtype;
+} pf_rope_axes_args;
+
+int pf_rope_axes(const pf_rope_axes_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged-pool write with the rotation on the way: pf_rope_axes of q (into
+ * q_out) and of k, whose rows then go to the page pool with those of v as
+ * pf_paged_cache_write writes them, in one launch. The reference rotates, then
+ * writes one token of one sequence (model.py:340-347; paged.py:205-223).
+ *   q, k, v: as q and k of pf_rope_axes (v: num_kv_heads)
+ *   q_out [batch, num_heads, seq_len, head_dim], dense
+ *   k_pages, v_pages, block_tables, positions, positions_stride: the pool, and
+ *     where row i of sequence b lands, as pf_paged_cache_write's
+ *   rope_positions: the rotary positions, as positions of pf_rope_axes; NULL
+ *     (axes = 1): the row's own position, positions[b] + i
+ *   seq_lens [batch] device int32 or NULL: rows at or past seq_lens[b] are
+ *     padding -- nothing is written to the pool, q_out is zero
+ * A row with a rotary position outside [0, rope_len) is treated as padding. A
+ * row without a page (as in pf_paged_cache_write) is not written, q_out is.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_pages;
+  void* v_pages;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, head, sequence */
+  const int32_t* block_tables;
+  const int32_t* positions;
+  int32_t positions_stride;
+  const int32_t* seq_lens;
+  const void* rope_positions;
+  int64_t rope_positions_stride[3]; /* axis, batch, sequence */
+  int32_t rope_positions_i64;
+  int32_t axes;
+  int32_t sections[PF_MAX_ROPE_AXES];
+  const float* cos;
+  const float* sin;
+  int32_t rope_len;
+  int32_t batch, num_heads, num_kv_heads, seq_len, num_pages, page_size, head_dim, pages_per_seq;
+  int32_t dtype;
+} pf_rope_paged_write_args;
+
+int pf_rope_paged_cache_write(const pf_rope_paged_write_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Fused decode step. Replaces the attention part of one decode_step /
  * ring_decode_step layer (model.py:340-347, :485-491): RoPE of the new
  * token's q and k at its position (rotate-half, float32, rounded once), the

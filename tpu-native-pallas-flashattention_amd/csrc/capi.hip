@@ -979,6 +979,92 @@ int pf_paged_cache_write(const pf_paged_cache_write_args* a, void* stream) {
   return finish(pf::launch_paged_cache_write(p, a->dtype, a->head_dim, (hipStream_t)stream));
 }
 
+// ---------------------------------------------------------------------------
+// Multi-axis rotary positions
+// ---------------------------------------------------------------------------
+// Axes, sections and tables, shared by the rotation and the append.
+static int fill_rope_axes(int32_t axes, const int32_t* sections, const float* cos, const float* sin, int32_t rope_len,
+                          int32_t batch, int32_t seq_len, int32_t head_dim, int32_t i64, int32_t dtype,
+                          pf::RopeAxesParams* p) {
+  static_assert(PF_MAX_ROPE_AXES == pf::kMaxRopeAxes, "axes of the C ABI and the kernel");
+  if (batch < 0 || seq_len < 0 || head_dim < 2 || head_dim % 2 != 0) return PF_ERR_INVALID;
+  if (axes < 1 || axes > PF_MAX_ROPE_AXES || (i64 != 0 && i64 != 1)) return PF_ERR_INVALID;
+  if (!cos || !sin || rope_len < 1) return PF_ERR_INVALID;
+  if (!dtype_ok(dtype)) return PF_ERR_UNSUPPORTED;
+  *p = pf::RopeAxesParams{};
+  int64_t end = 0;
+  for (int a = 0; a < axes; ++a) {
+    if (sections[a] < 1) return PF_ERR_INVALID;
+    end += sections[a];
+    p->ends[a] = (int)std::min(end, (int64_t)head_dim);
+  }
+  if (end != head_dim / 2) return PF_ERR_INVALID;
+  p->axes = axes;
+  p->cos = cos;
+  p->sin = sin;
+  p->rope_len = rope_len;
+  p->B = batch;
+  p->S = seq_len;
+  p->D = head_dim;
+  p->pos64 = i64;
+  return PF_OK;
+}
+
+static void set_rope_input(pf::RopeAxesParams* p, int i, const void* x, const int64_t* stride, int heads, void* out) {
+  p->x[i] = x;
+  p->sb[i] = stride[0];
+  p->sh[i] = stride[1];
+  p->ss[i] = stride[2];
+  p->heads[i] = heads;
+  p->out[i] = out;
+}
+
+int pf_rope_axes(const pf_rope_axes_args* a, void* stream) {
+  if (!a) return PF_ERR_INVALID;
+  pf::RopeAxesParams p;
+  const int st = fill_rope_axes(a->axes, a->sections, a->cos, a->sin, a->rope_len, a->batch, a->seq_len, a->head_dim,
+                                a->positions_i64, a->dtype, &p);
+  if (st != PF_OK) return st;
+  if (a->num_heads < 1 || a->num_kv_heads < 0 || (a->inverse != 0 && a->inverse != 1)) return PF_ERR_INVALID;
+  if ((int64_t)a->batch * a->seq_len == 0) return PF_OK;
+  if (!a->q || !a->q_out || !a->positions || (a->num_kv_heads > 0 && (!a->k || !a->k_out))) return PF_ERR_INVALID;
+  set_rope_input(&p, 0, a->q, a->q_stride, a->num_heads, a->q_out);
+  set_rope_input(&p, 1, a->k, a->k_stride, a->num_kv_heads, a->k_out);
+  p.positions = a->positions;
+  for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->positions_stride[i];
+  p.inverse = a->inverse;
+  return finish(pf::launch_rope_axes(p, a->dtype, false, (hipStream_t)stream));
+}
+
+int pf_rope_paged_cache_write(const pf_rope_paged_write_args* a, void* stream) {
+  if (!a) return PF_ERR_INVALID;
+  pf::RopeAxesParams p;
+  const int st = fill_rope_axes(a->axes, a->sections, a->cos, a->sin, a->rope_len, a->batch, a->seq_len, a->head_dim,
+                                a->rope_positions_i64, a->dtype, &p);
+  if (st != PF_OK) return st;
+  if (a->num_heads < 1 || a->num_kv_heads < 1 || a->num_pages < 1 || a->page_size < 1 || a->pages_per_seq < 0)
+    return PF_ERR_INVALID;
+  if (a->positions_stride != 0 && a->positions_stride != 1) return PF_ERR_INVALID;
+  if (!a->rope_positions && a->axes != 1) return PF_ERR_INVALID;
+  if ((int64_t)a->batch * a->seq_len == 0) return PF_OK;
+  if (!a->q || !a->k || !a->v || !a->q_out || !a->k_pages || !a->v_pages || !a->positions ||
+      (a->pages_per_seq > 0 && !a->block_tables))
+    return PF_ERR_INVALID;
+  set_rope_input(&p, 0, a->q, a->q_stride, a->num_heads, a->q_out);
+  set_rope_input(&p, 1, a->k, a->k_stride, a->num_kv_heads, a->k_pages);
+  set_rope_input(&p, 2, a->v, a->v_stride, a->num_kv_heads, a->v_pages);
+  p.positions = a->rope_positions;
+  for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->rope_positions_stride[i];
+  p.block_tables = a->block_tables;
+  p.position = a->positions;
+  p.position_stride = a->positions_stride;
+  p.seq_lens = a->seq_lens;
+  p.num_pages = a->num_pages;
+  p.page_size = a->page_size;
+  p.pages_per_seq = a->pages_per_seq;
+  return finish(pf::launch_rope_axes(p, a->dtype, true, (hipStream_t)stream));
+}
+
 // The fused decode step is one streaming-decode launch in its step mode
 // (decode_stream.hip, PG == 1) plus the combine; its workspace is the split
 // partials only.

@@ -348,4 +348,31 @@ struct PagedWriteParams {
 };
 hipError_t launch_paged_cache_write(const PagedWriteParams& p, int dtype, int head_dim, hipStream_t stream);
 
+// Multi-axis rotation of q and k, or rotation of q and append of k and v to a
+// paged pool (rope_axes.hip).
+constexpr int kMaxRopeAxes = 4;
+struct RopeAxesParams {
+  const void* x[3];  // q, k, v: [B, heads, S, D], strides (elements) of the first three dimensions
+  int64_t sb[3], sh[3], ss[3];
+  int heads[3];
+  void* out[3];           // q: [B, Hq, S, D]; k: the same with Hkv, or append: k and v pools
+  const void* positions;  // [axes, B, S] by strides; append: null = position[b] + s on the one axis
+  int64_t pos_stride[3];
+  int pos64;              // positions are int64 (else int32)
+  int axes;
+  int ends[kMaxRopeAxes];  // the pairs of axis a end at ends[a]
+  const float* cos;        // [rope_len, D]
+  const float* sin;
+  int rope_len;
+  int B, S, D;
+  int inverse;
+  // append
+  const int32_t* block_tables;  // [B, pages_per_seq]
+  const int32_t* position;      // row s of sequence b lands at position[b * position_stride] + s
+  int position_stride;
+  const int32_t* seq_lens;      // [B] or null: rows at or past it are skipped
+  int num_pages, page_size, pages_per_seq;
+};
+hipError_t launch_rope_axes(const RopeAxesParams& p, int dtype, bool append, hipStream_t stream);
+
 }  // namespace pf

@@ -13,10 +13,11 @@ not part of this package -- they are consumers of these functions.
 
 from .flash_attention import flash_attention, flash_attention_decode, flash_attention_with_lse
 from .fused_rope import flash_attention_rope
-from .paged import paged_flash_attention, init_paged_cache, write_to_paged_cache
+from .paged import paged_flash_attention, init_paged_cache, write_to_paged_cache, write_to_paged_cache_rope
 from .cache import flash_attention_decode_step, write_kv_cache, ring_kv_len
 from .reference import reference_attention
 from .rope import precompute_rope, apply_rope
+from .rope_axes import apply_rope_axes
 
 __all__ = [
     "flash_attention",
@@ -26,12 +27,14 @@ __all__ = [
     "paged_flash_attention",
     "init_paged_cache",
     "write_to_paged_cache",
+    "write_to_paged_cache_rope",
     "flash_attention_decode_step",
     "write_kv_cache",
     "ring_kv_len",
     "reference_attention",
     "precompute_rope",
     "apply_rope",
+    "apply_rope_axes",
 ]
 
 __version__ = "0.1.0"

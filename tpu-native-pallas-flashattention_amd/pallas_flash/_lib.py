@@ -26,6 +26,7 @@ PF_ERR_LAUNCH = -4
 PF_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 c_i32 = ctypes.c_int32
+c_i64 = ctypes.c_int64
 c_f32 = ctypes.c_float
 c_ptr = ctypes.c_void_p
 
@@ -104,6 +105,34 @@ class PagedWriteArgs(ctypes.Structure):
     ]
 
 
+MAX_ROPE_AXES = 4
+
+
+class RopeAxesArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_ptr), ("k", c_ptr), ("q_out", c_ptr), ("k_out", c_ptr),
+        ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3),
+        ("positions", c_ptr), ("positions_stride", c_i64 * 3), ("positions_i64", c_i32),
+        ("axes", c_i32), ("sections", c_i32 * MAX_ROPE_AXES),
+        ("cos", c_ptr), ("sin", c_ptr), ("rope_len", c_i32),
+        ("batch", c_i32), ("num_heads", c_i32), ("num_kv_heads", c_i32), ("seq_len", c_i32), ("head_dim", c_i32),
+        ("inverse", c_i32), ("dtype", c_i32),
+    ]
+
+
+class RopePagedWriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_ptr), ("k", c_ptr), ("v", c_ptr), ("q_out", c_ptr), ("k_pages", c_ptr), ("v_pages", c_ptr),
+        ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+        ("block_tables", c_ptr), ("positions", c_ptr), ("positions_stride", c_i32), ("seq_lens", c_ptr),
+        ("rope_positions", c_ptr), ("rope_positions_stride", c_i64 * 3), ("rope_positions_i64", c_i32),
+        ("axes", c_i32), ("sections", c_i32 * MAX_ROPE_AXES),
+        ("cos", c_ptr), ("sin", c_ptr), ("rope_len", c_i32),
+        ("batch", c_i32), ("num_heads", c_i32), ("num_kv_heads", c_i32), ("seq_len", c_i32), ("num_pages", c_i32),
+        ("page_size", c_i32), ("head_dim", c_i32), ("pages_per_seq", c_i32), ("dtype", c_i32),
+    ]
+
+
 class DecodeStepArgs(ctypes.Structure):
     _fields_ = [
         ("q", c_ptr), ("k_new", c_ptr), ("v_new", c_ptr), ("k_cache", c_ptr), ("v_cache", c_ptr),
@@ -142,6 +171,8 @@ SIGNATURES = {
     "pf_rope": ([ctypes.POINTER(RopeArgs), c_ptr], ctypes.c_int),
     "pf_kv_cache_write": ([ctypes.POINTER(KvWriteArgs), c_ptr], ctypes.c_int),
     "pf_paged_cache_write": ([ctypes.POINTER(PagedWriteArgs), c_ptr], ctypes.c_int),
+    "pf_rope_axes": ([ctypes.POINTER(RopeAxesArgs), c_ptr], ctypes.c_int),
+    "pf_rope_paged_cache_write": ([ctypes.POINTER(RopePagedWriteArgs), c_ptr], ctypes.c_int),
     "pf_attn_decode_step_workspace_size": ([ctypes.POINTER(DecodeStepArgs)], ctypes.c_size_t),
     "pf_attn_decode_step": ([ctypes.POINTER(DecodeStepArgs), c_ptr], ctypes.c_int),
     "pf_get_tuning": ([ctypes.POINTER(Tuning)], ctypes.c_int),

@@ -18,7 +18,7 @@ regardless, paged.py:119-121).
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -176,4 +176,108 @@ def write_to_paged_cache(k_pages, v_pages, k, v, block_table, position, *, inpla
     return k_pages, v_pages
 
 
-__all__ = ["paged_flash_attention", "init_paged_cache", "write_to_paged_cache"]
+def write_to_paged_cache_rope(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    block_table,
+    position,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    *,
+    rope_positions=None,
+    sections: Optional[Sequence[int]] = None,
+    seq_lens=None,
+):
+    """Rotate the new tokens' q and k and write k and v into their pages, in
+    one launch (pf_rope_paged_cache_write): the part of a layer between its
+    projections and ``paged_flash_attention``. The reference rotates first
+    (model.py:340-341) and writes one token of one sequence (paged.py:205-223).
+
+    Args:
+        k_pages, v_pages: ``[num_pages, num_kv_heads, page_size, head_dim]``,
+            written in place.
+        q: ``[batch, num_heads, seq_len, head_dim]``, before RoPE.
+        k, v: ``[batch, num_kv_heads, seq_len, head_dim]``, k before RoPE. All
+            of one dtype; read with their own strides (views of one fused
+            projection are not copied).
+        block_table, position: as ``write_to_paged_cache``: row ``i`` of
+            sequence ``b`` lands at position ``position[b] + i`` of its table;
+            a row without a page there is not written.
+        cos, sin: ``[rope_len, head_dim]`` tables (``precompute_rope``).
+        rope_positions: the rotary positions where they are not the rows' own
+            ``position[b] + i`` (several axes; tokens behind a shared prefix):
+            integers ``[axes, seq_len]`` or ``[axes, batch, seq_len]`` as
+            ``apply_rope_axes`` takes them. A row with one outside the tables
+            writes nothing, its q is zero.
+        sections: the rotated pairs of each axis (``apply_rope_axes``); several
+            axes need ``rope_positions``.
+        seq_lens: ``[batch]`` integers: rows at or past them are padding --
+            nothing is written, q is zero. ``None``: all rows are tokens.
+
+    Returns ``(q_rot, k_pages, v_pages)``: the rotated q, dense, and the pools.
+    No gradients: the pools belong to inference.
+    """
+    from .cache import _check_positions, _positions
+    from .rope_axes import (check_axis_positions, check_sections, check_tables, device_positions, rows_of, sections4,
+                            strides3)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be [num_pages, num_kv_heads, page_size, head_dim] of one shape")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("q must be [batch, num_heads, seq_len, head_dim], k and v [batch, num_kv_heads, seq_len, "
+                         "head_dim] of one shape")
+    num_pages, hkv, page_size, d = k_pages.shape
+    batch, hq, seq, _ = q.shape
+    if k.shape[1] != hkv or k.shape[3] != d or num_pages == 0 or page_size == 0:
+        raise ValueError(f"k {tuple(k.shape)} does not match the pool {tuple(k_pages.shape)}")
+    if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must share batch, seq_len and head_dim")
+    if hkv == 0 or hq == 0 or hq % hkv != 0:
+        raise ValueError(f"num_heads ({hq}) must be a multiple of num_kv_heads ({hkv})")
+    if any(t.dtype != k_pages.dtype for t in (v_pages, q, k, v)):
+        raise ValueError("q, k, v and the pools must share a dtype")
+    sections = check_sections(sections, d)
+    check_tables(cos, sin, d)
+    if rope_positions is not None:
+        rope_positions = check_axis_positions(rope_positions, len(sections), batch, seq)
+    elif len(sections) > 1:
+        raise ValueError("several axes need rope_positions")
+    table = torch.as_tensor(block_table)
+    if table.dim() == 1:
+        table = table.unsqueeze(0)
+    if table.dim() != 2 or table.shape[0] != batch:
+        raise ValueError(f"block_table must be [pages_per_seq] or [batch, pages_per_seq], got {tuple(table.shape)}")
+    _check_positions(position, batch)
+    if seq_lens is not None:
+        seq_lens = torch.as_tensor(seq_lens)
+        if tuple(seq_lens.shape) != (batch,) or seq_lens.dtype.is_floating_point or seq_lens.dtype == torch.bool:
+            raise ValueError(f"seq_lens must be [batch] integers, got {tuple(seq_lens.shape)} {seq_lens.dtype}")
+    _lib.require_device(k_pages, v_pages, q, k, v)
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("the page pools are written in place and must be contiguous")
+    dev = k_pages.device
+    q_rot = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if q_rot.numel() == 0:
+        return q_rot, k_pages, v_pages
+    q, k, v = (rows_of(t.detach()) for t in (q, k, v))
+    table = table.to(device=dev, dtype=torch.int32).contiguous()
+    pos, stride = _positions(position, batch, dev)
+    if seq_lens is not None:
+        seq_lens = seq_lens.to(device=dev, dtype=torch.int32).contiguous()
+    rope, rope_stride, i64 = None, (0, 0, 0), 0
+    if rope_positions is not None:
+        rope, rope_stride, i64 = device_positions(rope_positions, dev)
+    cos, sin = (t.detach().to(device=dev, dtype=torch.float32).contiguous() for t in (cos, sin))
+    args = _lib.RopePagedWriteArgs(
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(q_rot), _lib.ptr(k_pages), _lib.ptr(v_pages), strides3(q),
+        strides3(k), strides3(v), _lib.ptr(table), _lib.ptr(pos), stride, _lib.ptr(seq_lens), _lib.ptr(rope),
+        (_lib.c_i64 * 3)(*rope_stride), i64, len(sections), sections4(sections), _lib.ptr(cos), _lib.ptr(sin),
+        cos.shape[0], batch, hq, hkv, seq, num_pages, page_size, d, table.shape[1], _lib.dtype_tag(k_pages))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().pf_rope_paged_cache_write(args, _lib.stream_of(k_pages)), "write_to_paged_cache_rope")
+    return q_rot, k_pages, v_pages
+
+
+__all__ = ["paged_flash_attention", "init_paged_cache", "write_to_paged_cache", "write_to_paged_cache_rope"]
