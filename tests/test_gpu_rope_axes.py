@@ -345,3 +345,32 @@ def test_append_empty():
     before = kp.clone()
     q1, _, _ = write_to_paged_cache_rope(kp, vp, q[:, :, :0], k[:, :, :0], v[:, :, :0], table, 0, cos, sin)
     assert q1.shape == (2, 4, 0, 64) and torch.equal(kp, before)
+
+
+@pytest.mark.parametrize("dt,hq,hk,d", [("bf16", 15, 5, 128), ("f32", 6, 3, 64), ("f16", 7, 7, 256)])
+def test_large_calls(dt, hq, hk, d):
+    """Past 48 MB a thread takes four heads: the bits of the same call in short pieces, head counts that four does not divide."""
+    s = 26000000 // ((hq + hk) * d * 2 * torch.finfo(TORCH_DT[dt]).bits // 8) + 7
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(2, s, hq + 2 * hk, d, device="cuda", generator=gen).to(TORCH_DT[dt]).transpose(1, 2)
+    q, k, v = x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:]
+    cos, sin = tables(300, d)
+    sections = (d // 8, d // 4, d // 8)
+    pos = torch.randint(-1, 300, (3, 2, s), device="cuda", generator=gen)
+    page, per = 64, -(-(s + 5) // 64)
+    table = torch.randperm(2 * per, device="cuda", generator=gen).to(torch.int32).view(2, per)
+    pools = [torch.zeros(2 * per, hk, page, d, device="cuda", dtype=x.dtype) for _ in range(4)]
+    lens = torch.tensor([s - 11, 1500], device="cuda", dtype=torch.int32)
+    qr, kr = apply_rope_axes(q, k, pos, cos, sin, sections)
+    qa, _, _ = write_to_paged_cache_rope(*pools[:2], q, k, v, table, 5, cos, sin, rope_positions=pos,
+                                         sections=sections, seq_lens=lens)
+    for lo in range(0, s, 1000):
+        at = slice(lo, lo + 1000)
+        q1, k1 = apply_rope_axes(q[:, :, at], k[:, :, at], pos[:, :, at], cos, sin, sections)
+        assert torch.equal(q1, qr[:, :, at]) and torch.equal(k1, kr[:, :, at])
+        q1, _, _ = write_to_paged_cache_rope(*pools[2:], q[:, :, at], k[:, :, at], v[:, :, at], table, 5 + lo, cos,
+                                             sin, rope_positions=pos[:, :, at], sections=sections, seq_lens=lens - lo)
+        assert torch.equal(q1, qa[:, :, at])
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+    keep = (pos >= 0).all(0)[:, None, :, None] & (torch.arange(s, device="cuda") < lens[:, None])[:, None, :, None]
+    assert torch.equal(qa, torch.where(keep, qr, torch.zeros_like(qr))) and pools[0].any()

@@ -993,10 +993,12 @@ static int fill_rope_axes(int32_t axes, const int32_t* sections, const float* co
   if (!dtype_ok(dtype)) return PF_ERR_UNSUPPORTED;
   *p = pf::RopeAxesParams{};
   int64_t end = 0;
-  for (int a = 0; a < axes; ++a) {
-    if (sections[a] < 1) return PF_ERR_INVALID;
-    end += sections[a];
-    p->ends[a] = (int)std::min(end, (int64_t)head_dim);
+  for (int a = 0; a < PF_MAX_ROPE_AXES; ++a) {
+    if (a < axes) {
+      if (sections[a] < 1) return PF_ERR_INVALID;
+      end += sections[a];
+    }
+    p->ends[a] = a < axes - 1 ? (int)std::min(end, (int64_t)head_dim) : head_dim;
   }
   if (end != head_dim / 2) return PF_ERR_INVALID;
   p->axes = axes;

@@ -351,6 +351,10 @@ hipError_t launch_paged_cache_write(const PagedWriteParams& p, int dtype, int he
 // Multi-axis rotation of q and k, or rotation of q and append of k and v to a
 // paged pool (rope_axes.hip).
 constexpr int kMaxRopeAxes = 4;
+struct FastDiv {
+  uint32_t d, mul;
+  int shift;
+};
 struct RopeAxesParams {
   const void* x[3];  // q, k, v: [B, heads, S, D], strides (elements) of the first three dimensions
   int64_t sb[3], sh[3], ss[3];
@@ -360,7 +364,7 @@ struct RopeAxesParams {
   int64_t pos_stride[3];
   int pos64;              // positions are int64 (else int32)
   int axes;
-  int ends[kMaxRopeAxes];  // the pairs of axis a end at ends[a]
+  int ends[kMaxRopeAxes];  // the pairs of axis a end at ends[a]; from the last axis on: head_dim (past every pair)
   const float* cos;        // [rope_len, D]
   const float* sin;
   int rope_len;
@@ -372,6 +376,12 @@ struct RopeAxesParams {
   int position_stride;
   const int32_t* seq_lens;      // [B] or null: rows at or past it are skipped
   int num_pages, page_size, pages_per_seq;
+  // the launch's own (rope_axes.hip): (batch, token, chunk) items of tokens s0
+  // on, head groups of each tensor, divisors
+  uint32_t n_items;
+  int s0;
+  int groups[3];
+  FastDiv div_chunks, div_seq, div_page;
 };
 hipError_t launch_rope_axes(const RopeAxesParams& p, int dtype, bool append, hipStream_t stream);
 

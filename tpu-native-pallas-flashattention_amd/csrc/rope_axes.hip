@@ -24,21 +24,22 @@
 #include "pf_common.hpp"
 #include "pf_kernels.hpp"
 
+#include <algorithm>
+
 namespace pf {
 
 namespace {
 
-// a / b and a % b for a >= 0, in 32 bits where they do (a 64-bit division is
-// several hundred instructions).
-__device__ inline int64_t divmod(int64_t a, int b, int* rem) {
-  if (((uint64_t)a >> 32) == 0) {
-    const uint32_t q = (uint32_t)a / (uint32_t)b;
-    *rem = (int)((uint32_t)a - q * (uint32_t)b);
-    return q;
-  }
-  const int64_t q = a / b;
-  *rem = (int)(a - q * b);
-  return q;
+// n / d of n < 2^31 by the divisor's multiplier (fast_divisor): with l =
+// ceil(log2 d) and m = floor(2^(31 + l) / d) + 1 < 2^32, n m / 2^(31 + l) lies
+// less than 1 / d above n / d.
+__device__ inline uint32_t fast_div(uint32_t n, const FastDiv& f) {
+  return (uint32_t)(((uint64_t)n * f.mul) >> f.shift);
+}
+FastDiv fast_divisor(int d) {
+  int l = 0;
+  while (((int64_t)1 << l) < d) ++l;
+  return FastDiv{(uint32_t)d, (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)d) + 1), 31 + l};
 }
 
 // E elements, element-aligned: rows need no 16-byte alignment.
@@ -55,89 +56,128 @@ __device__ inline void load_table(const float* t, float* out) {
   for (int e = 0; e < E; ++e) out[e] = x[e];
 }
 
-__device__ inline int64_t position(const RopeAxesParams& p, int axis, int b, int s) {
-  const int64_t at = axis * p.pos_stride[0] + b * p.pos_stride[1] + s * p.pos_stride[2];
-  return p.pos64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
+// Entry `which` of a parameter's three: by selects, as an indexed read would
+// keep the parameters in scratch memory.
+template <typename V>
+__device__ inline V pick(const V (&v)[3], int which) {
+  V x = v[0];
+  if (which == 1) x = v[1];
+  if (which == 2) x = v[2];
+  return x;
+}
+
+// A token's table rows, one for each axis, in a vector (a struct or an array
+// of them goes to LDS for the choices of row_of), and whether all of them lie
+// inside the tables.
+template <typename I>
+__device__ inline i32x4 axis_rows(const RopeAxesParams& p, int b, int s, bool* inside) {
+  static_assert(kMaxRopeAxes == 4, "four rows");
+  const I* at = static_cast<const I*>(p.positions) + b * p.pos_stride[1] + s * p.pos_stride[2];
+  const uint64_t n = p.rope_len;
+  auto in = [&](I pos) { return (uint64_t)(int64_t)pos < n; };  // and not negative
+  if (p.axes == 1) {
+    const I x = at[0];
+    *inside = in(x);
+    return (i32x4){(int)x, 0, 0, 0};
+  }
+  // all four at once (those past the last axis repeat it), not one after another
+  const int last = p.axes - 1;
+  const I x0 = at[0], x1 = at[p.pos_stride[0]], x2 = at[min(2, last) * p.pos_stride[0]],
+          x3 = at[last * p.pos_stride[0]];
+  *inside = (bool)(in(x0) & in(x1) & in(x2) & in(x3));
+  return (i32x4){(int)x0, (int)x1, (int)x2, (int)x3};
+}
+// The row of pair i. ends[a] is past every pair from the last axis on.
+__device__ inline int row_of(const RopeAxesParams& p, const i32x4& rows, int i) {
+  int r = rows[0];
+  if (i >= p.ends[0]) r = rows[1];
+  if (i >= p.ends[1]) r = rows[2];
+  if (i >= p.ends[2]) r = rows[3];
+  return r;
+}
+
+template <typename T, int E, bool NT>
+__device__ inline typename Vec<T, E>::type get(const T* a) {
+  typedef typename Vec<T, E>::type vT;
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const vT*>(a));
+  else return *reinterpret_cast<const vT*>(a);
+}
+template <typename T, int E, bool NT>
+__device__ inline void put(T* a, typename Vec<T, E>::type v) {
+  typedef typename Vec<T, E>::type vT;
+  if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<vT*>(a));
+  else *reinterpret_cast<vT*>(a) = v;
 }
 
 template <typename T, int E, int NH, bool APPEND>
-__global__ __launch_bounds__(256) void pf_rope_axes_kernel(RopeAxesParams p, int64_t n_items) {
+__global__ __launch_bounds__(256) void pf_rope_axes_kernel(RopeAxesParams p) {
   typedef typename Vec<T, E>::type vT;
-  const int half = p.D / 2, HC = half / E;
-  int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (it >= n_items) return;
-  int c, s, hg;
-  it = divmod(it, HC, &c);
-  it = divmod(it, p.S, &s);
-  const int n_grp[3] = {(p.heads[0] + NH - 1) / NH, (p.heads[1] + NH - 1) / NH, APPEND ? (p.heads[2] + NH - 1) / NH : 0};
-  const int b = (int)divmod(it, n_grp[0] + n_grp[1] + n_grp[2], &hg);
-  int which = 0;  // q, k, v
-  if (hg >= n_grp[0]) {
-    hg -= n_grp[0];
+  constexpr bool NT = NH > 1;
+  const int half = p.D / 2;
+  // blockIdx.y: the tensor (q, k, v) and its head group -- uniform, so that
+  // bases and strides are scalars; x: (batch, token, chunk).
+  int hg = blockIdx.y, which = 0;
+  if (hg >= p.groups[0]) {
+    hg -= p.groups[0];
     which = 1;
-    if (APPEND && hg >= n_grp[1]) {
-      hg -= n_grp[1];
+    if (APPEND && hg >= p.groups[1]) {
+      hg -= p.groups[1];
       which = 2;
     }
   }
-  const int h0 = hg * NH, heads = p.heads[which], nh = min(NH, heads - h0);
+  const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+  if (item >= p.n_items) return;
+  const uint32_t tok = fast_div(item, p.div_chunks);
+  const int c = (int)(item - tok * p.div_chunks.d);
+  const uint32_t bt = fast_div(tok, p.div_seq);
+  const int b = (int)bt, s = p.s0 + (int)(tok - bt * p.div_seq.d);
+  const int h0 = hg * NH, heads = pick(p.heads, which), nh = min(NH, heads - h0);
   const int i0 = c * E;  // the thread's first pair
 
+  // Lookups first, the rows of x behind them: loads complete in order, so the
+  // table loads that need the lookups wait for nothing else.
   bool live = true;
   int64_t own = 0;  // append: the token's position in its sequence
+  i32x4 rows;
+  bool inside;
   if constexpr (APPEND) {
-    live = p.seq_lens == nullptr || s < p.seq_lens[b];
     own = (int64_t)p.position[(int64_t)b * p.position_stride] + s;
+    live = p.seq_lens == nullptr || s < p.seq_lens[b];
   }
-  // The input does not depend on the lookups: under way beside them.
-  const T* src = static_cast<const T*>(p.x[which]) + b * p.sb[which] + h0 * p.sh[which] + s * p.ss[which] + i0;
+  if (APPEND && p.positions == nullptr) {
+    rows = (i32x4){(int)own, 0, 0, 0};
+    inside = own >= 0 && own < p.rope_len;
+  } else {
+    rows = p.pos64 ? axis_rows<int64_t>(p, b, s, &inside) : axis_rows<int32_t>(p, b, s, &inside);
+  }
+
+  const int64_t sh = pick(p.sh, which);
+  const T* src = static_cast<const T*>(pick(p.x, which)) + h0 * sh + b * pick(p.sb, which) + s * pick(p.ss, which) + i0;
   vT lo[NH], hi[NH];
   if (live) {
 #pragma unroll
     for (int j = 0; j < NH; ++j)
       if (j < nh) {
-        lo[j] = __builtin_nontemporal_load(reinterpret_cast<const vT*>(src + j * p.sh[which]));
-        hi[j] = __builtin_nontemporal_load(reinterpret_cast<const vT*>(src + j * p.sh[which] + half));
+        lo[j] = get<T, E, NT>(src + j * sh);
+        hi[j] = get<T, E, NT>(src + j * sh + half);
       }
   }
-
-  // The table rows of the first and last pair's axis; ends[] covers all pairs.
-  int64_t row0 = own, row1 = own;
-  int a0 = 0, a1 = 0;
-  if (live) {
-    if (!APPEND || p.positions != nullptr) {
-#pragma unroll
-      for (int a = 0; a < kMaxRopeAxes; ++a) {
-        if (a >= p.axes) break;
-        const int64_t pos = position(p, a, b, s);
-        live = live && pos >= 0 && pos < p.rope_len;
-        if (a == 0 || i0 >= p.ends[a - 1]) {
-          row0 = pos;
-          a0 = a;
-        }
-        if (a == 0 || i0 + E - 1 >= p.ends[a - 1]) {
-          row1 = pos;
-          a1 = a;
-        }
-      }
-    } else {
-      live = own >= 0 && own < p.rope_len;
-    }
-  }
+  live = live && inside;
 
   // Where the rows go; pools: only where the position has a page.
   T* dst = nullptr;
   int64_t step = 0;  // from head to head
   if (!APPEND || which == 0) {
-    dst = static_cast<T*>(p.out[which]) + (((int64_t)b * heads + h0) * p.S + s) * p.D + i0;
+    dst = static_cast<T*>(pick(p.out, which)) + (((int64_t)b * heads + h0) * p.S + s) * p.D + i0;
     step = (int64_t)p.S * p.D;
   } else if (live && own >= 0) {
-    int off;
-    const int64_t lp = divmod(own, p.page_size, &off);
-    if (lp < p.pages_per_seq) {
+    // own < 2^31 wherever it has a page
+    const uint32_t lp = (uint64_t)own >> 31 ? ~0u : fast_div((uint32_t)own, p.div_page);
+    if (lp < (uint32_t)p.pages_per_seq) {
       const int page = p.block_tables[(int64_t)b * p.pages_per_seq + lp];
+      const int off = (int)own - (int)lp * p.page_size;
       if (page >= 0 && page < p.num_pages) {
-        dst = static_cast<T*>(p.out[which]) +
+        dst = static_cast<T*>(pick(p.out, which)) +
               (((int64_t)page * heads + h0) * p.page_size + off) * p.D + i0;
         step = (int64_t)p.page_size * p.D;
       }
@@ -149,8 +189,8 @@ __global__ __launch_bounds__(256) void pf_rope_axes_kernel(RopeAxesParams p, int
 #pragma unroll
     for (int j = 0; j < NH; ++j)
       if (j < nh) {
-        *reinterpret_cast<vT*>(dst + j * step) = lo[j];
-        *reinterpret_cast<vT*>(dst + j * step + half) = hi[j];
+        put<T, E, NT>(dst + j * step, lo[j]);
+        put<T, E, NT>(dst + j * step + half, hi[j]);
       }
     return;
   }
@@ -158,16 +198,20 @@ __global__ __launch_bounds__(256) void pf_rope_axes_kernel(RopeAxesParams p, int
 #pragma unroll
     for (int j = 0; j < NH; ++j)
       if (j < nh) {
-        *reinterpret_cast<vT*>(dst + j * step) = (vT)(Elem<T>::from_f32(0.f));
-        *reinterpret_cast<vT*>(dst + j * step + half) = (vT)(Elem<T>::from_f32(0.f));
+        put<T, E, NT>(dst + j * step, (vT)(Elem<T>::from_f32(0.f)));
+        put<T, E, NT>(dst + j * step + half, (vT)(Elem<T>::from_f32(0.f)));
       }
     return;
   }
 
   float c1[E], c2[E], s1[E], s2[E];
-  if (a0 == a1) {
-    const float* cr = p.cos + row0 * p.D + i0;
-    const float* sr = p.sin + row0 * p.D + i0;
+  const int row = row_of(p, rows, i0);
+  bool cut = false;  // an axis ends inside the thread's pairs
+#pragma unroll
+  for (int a = 0; a < kMaxRopeAxes - 1; ++a) cut = cut || (i0 < p.ends[a] && p.ends[a] < i0 + E);
+  if (!cut) {
+    const float* cr = p.cos + (int64_t)row * p.D + i0;
+    const float* sr = p.sin + (int64_t)row * p.D + i0;
     load_table<E>(cr, c1);
     load_table<E>(cr + half, c2);
     load_table<E>(sr, s1);
@@ -175,19 +219,11 @@ __global__ __launch_bounds__(256) void pf_rope_axes_kernel(RopeAxesParams p, int
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      int64_t row = row0;
-      if (i0 + e >= p.ends[a1 - 1]) row = row1;
-      else if (a1 > a0 + 1 && i0 + e >= p.ends[a0]) {  // an axis that lies inside the thread's pairs
-        int a = a0 + 1;
-        while (i0 + e >= p.ends[a]) ++a;
-        row = position(p, a, b, s);
-      }
-      const float* cr = p.cos + row * p.D + i0 + e;
-      const float* sr = p.sin + row * p.D + i0 + e;
-      c1[e] = cr[0];
-      c2[e] = cr[half];
-      s1[e] = sr[0];
-      s2[e] = sr[half];
+      const int64_t at = (int64_t)row_of(p, rows, i0 + e) * p.D + i0 + e;
+      c1[e] = p.cos[at];
+      c2[e] = p.cos[at + half];
+      s1[e] = p.sin[at];
+      s2[e] = p.sin[at + half];
     }
   }
   if (p.inverse) {
@@ -209,24 +245,54 @@ __global__ __launch_bounds__(256) void pf_rope_axes_kernel(RopeAxesParams p, int
         y1[e] = Elem<T>::from_f32(fmaf(x1, c1[e], -(x2 * s1[e])));
         y2[e] = Elem<T>::from_f32(fmaf(x2, c2[e], x1 * s2[e]));
       }
-      *reinterpret_cast<vT*>(dst + j * step) = y1;
-      *reinterpret_cast<vT*>(dst + j * step + half) = y2;
+      put<T, E, NT>(dst + j * step, y1);
+      put<T, E, NT>(dst + j * step + half, y2);
     }
 }
 
 template <typename T, int E, int NH, bool APPEND>
-hipError_t launch_heads(const RopeAxesParams& p, hipStream_t st) {
-  int64_t grps = 0;
-  for (int w = 0; w < (APPEND ? 3 : 2); ++w) grps += (p.heads[w] + NH - 1) / NH;
-  const int64_t n = (int64_t)p.B * p.S * grps * (p.D / 2 / E);
-  const int64_t grid = (n + 255) / 256;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((pf_rope_axes_kernel<T, E, NH, APPEND>), dim3((unsigned)grid), dim3(256), 0, st, p, n);
-  return hipGetLastError();
+hipError_t launch_heads(RopeAxesParams p, hipStream_t st) {
+  const int chunks = p.D / 2 / E;
+  unsigned groups = 0;
+  for (int w = 0; w < 3; ++w) {
+    p.groups[w] = w < (APPEND ? 3 : 2) ? (p.heads[w] + NH - 1) / NH : 0;
+    groups += p.groups[w];
+  }
+  p.div_chunks = fast_divisor(chunks);
+  p.div_page = fast_divisor(APPEND ? p.page_size : 1);
+  // 32-bit items: past 2^31 of them, the tokens in several launches.
+  const int64_t most = (((int64_t)1 << 31) - 256) / ((int64_t)p.B * chunks);
+  if (most < 1 || groups > 65535) return hipErrorInvalidValue;
+  const int seq = p.S;
+  for (int s0 = 0; s0 < seq; s0 += (int)std::min<int64_t>(most, seq)) {
+    const int n = (int)std::min<int64_t>(most, seq - s0);
+    p.s0 = s0;
+    p.div_seq = fast_divisor(n);
+    p.n_items = (uint32_t)((int64_t)p.B * n * chunks);
+    hipLaunchKernelGGL((pf_rope_axes_kernel<T, E, NH, APPEND>), dim3((p.n_items + 255) / 256, groups), dim3(256), 0,
+                       st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || n == seq - s0) return e;
+  }
+  return hipSuccess;
 }
 
+// Calls that move kStreamBytes or more run four heads a thread with
+// non-temporal loads and stores, smaller ones a head a thread (as many waves as
+// there can be) through the caches, where what reads the result next finds it.
+// Only for whole 16-byte chunks. (Strided inputs, forward: 32768 tokens, 32 + 8
+// float16 heads of 128, 671 MB: 170 us with a head a thread, 137 with four, 121
+// = 5.8 TB/s with four and non-temporal; a float32 step of 37 MB a launch: 8.7,
+// 9.0 and 10.1 us; 8 tokens: 3.0 and 3.4 us. On one shape the two forms cross at
+// 40-60 MB.)
+constexpr int64_t kStreamBytes = (int64_t)48 << 20;
 template <typename T, int E, bool APPEND>
 hipError_t launch_pairs(const RopeAxesParams& p, hipStream_t st) {
+  if constexpr (E * sizeof(T) == 16) {
+    const int64_t bytes =
+        (int64_t)p.B * p.S * (p.heads[0] + p.heads[1] + (APPEND ? p.heads[2] : 0)) * p.D * 2 * (int)sizeof(T);
+    if (bytes >= kStreamBytes) return launch_heads<T, E, 4, APPEND>(p, st);
+  }
   return launch_heads<T, E, 1, APPEND>(p, st);
 }
 
