@@ -318,6 +318,50 @@ int pf_paged_attn(const pf_paged_attn_args* args, void* stream);
 int pf_paged_attn_noalloc(const pf_paged_attn_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged single-query attention of a batch that shares a prefix: sequence b
+ * attends the prefix's keys and then its own, the prefix's pages being read
+ * once for the whole batch instead of once per sequence. No counterpart in the
+ * reference (its paged call, paged.py:102-192, would have the prefix's pages in
+ * every sequence's table).
+ *   q [batch, num_heads, 1, head_dim]; o same shape
+ *   k_pages, v_pages [num_pages, num_kv_heads, page_size, head_dim]
+ *   prefix_table [prefix_pages] int32 (device): the prefix's pages
+ *   prefix_len: its keys, in [0, prefix_pages * page_size]; the last page need
+ *     not be full
+ *   prefix_len_ptr: device int32 or NULL; given, the prefix has
+ *     max(0, min(*prefix_len_ptr, prefix_len)) keys (a captured call can follow
+ *     a prefix that grows)
+ *   block_tables [batch, pages_per_seq], context_lens [batch] int32 (device):
+ *     the sequences' own pages and keys, the prefix not counted
+ * Sequence b attends prefix + min(context_lens[b], pages_per_seq * page_size)
+ * keys; none at all gives o = 0. Table entries, head_dim and page_size as
+ * pf_paged_attn.
+ * workspace: at least pf_paged_prefix_attn_workspace_size(args) bytes, 256-byte
+ * aligned device memory (contents on entry do not matter). The size depends on
+ * the shapes, prefix_len and the alignment of q, k_pages and v_pages, not on
+ * what the device holds; 0: the call would be refused.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* prefix_table;
+  const int32_t* prefix_len_ptr;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  void* o;
+  int32_t batch, num_heads, num_kv_heads, num_pages, page_size, head_dim;
+  int32_t prefix_pages, prefix_len, pages_per_seq;
+  float sm_scale;
+  int32_t dtype;
+  void* workspace;
+  size_t workspace_bytes;
+} pf_paged_prefix_attn_args;
+
+size_t pf_paged_prefix_attn_workspace_size(const pf_paged_prefix_attn_args* args);
+int pf_paged_prefix_attn(const pf_paged_prefix_attn_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
  * KV-cache writes on device. Replaces the decode loop's `_cache_write`
  * (model.py:257-262, called at :299, :342, :487) and the ring-buffer slot
  * scatter of prefill_ring (model.py:437, :447-448) / ring_decode_step

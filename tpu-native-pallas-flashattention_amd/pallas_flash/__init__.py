@@ -13,7 +13,8 @@ not part of this package -- they are consumers of these functions.
 
 from .flash_attention import flash_attention, flash_attention_decode, flash_attention_with_lse
 from .fused_rope import flash_attention_rope
-from .paged import paged_flash_attention, init_paged_cache, write_to_paged_cache, write_to_paged_cache_rope
+from .paged import (paged_flash_attention, paged_flash_attention_prefix, init_paged_cache, write_to_paged_cache,
+                    write_to_paged_cache_rope)
 from .cache import flash_attention_decode_step, write_kv_cache, ring_kv_len
 from .reference import reference_attention
 from .rope import precompute_rope, apply_rope
@@ -25,6 +26,7 @@ __all__ = [
     "flash_attention_with_lse",
     "flash_attention_rope",
     "paged_flash_attention",
+    "paged_flash_attention_prefix",
     "init_paged_cache",
     "write_to_paged_cache",
     "write_to_paged_cache_rope",

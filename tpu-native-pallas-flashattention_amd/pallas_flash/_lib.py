@@ -79,6 +79,17 @@ class PagedArgs(ctypes.Structure):
     ]
 
 
+class PagedPrefixArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_ptr), ("k_pages", c_ptr), ("v_pages", c_ptr), ("prefix_table", c_ptr), ("prefix_len_ptr", c_ptr),
+        ("block_tables", c_ptr), ("context_lens", c_ptr), ("o", c_ptr),
+        ("batch", c_i32), ("num_heads", c_i32), ("num_kv_heads", c_i32),
+        ("num_pages", c_i32), ("page_size", c_i32), ("head_dim", c_i32),
+        ("prefix_pages", c_i32), ("prefix_len", c_i32), ("pages_per_seq", c_i32), ("sm_scale", c_f32),
+        ("dtype", c_i32), ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class RopeArgs(ctypes.Structure):
     _fields_ = [
         ("x", c_ptr), ("out", c_ptr), ("cos", c_ptr), ("sin", c_ptr),
@@ -168,6 +179,8 @@ SIGNATURES = {
     "pf_paged_attn_workspace_min": ([ctypes.POINTER(PagedArgs)], ctypes.c_size_t),
     "pf_paged_attn": ([ctypes.POINTER(PagedArgs), c_ptr], ctypes.c_int),
     "pf_paged_attn_noalloc": ([ctypes.POINTER(PagedArgs), c_ptr], ctypes.c_int),
+    "pf_paged_prefix_attn_workspace_size": ([ctypes.POINTER(PagedPrefixArgs)], ctypes.c_size_t),
+    "pf_paged_prefix_attn": ([ctypes.POINTER(PagedPrefixArgs), c_ptr], ctypes.c_int),
     "pf_rope": ([ctypes.POINTER(RopeArgs), c_ptr], ctypes.c_int),
     "pf_kv_cache_write": ([ctypes.POINTER(KvWriteArgs), c_ptr], ctypes.c_int),
     "pf_paged_cache_write": ([ctypes.POINTER(PagedWriteArgs), c_ptr], ctypes.c_int),

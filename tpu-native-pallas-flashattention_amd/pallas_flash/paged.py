@@ -18,6 +18,7 @@ regardless, paged.py:119-121).
 
 from __future__ import annotations
 
+import operator
 from typing import Optional, Sequence
 
 import torch
@@ -107,6 +108,102 @@ def paged_flash_attention(
     args.workspace_bytes = ws.numel()
     with torch.cuda.device(dev):
         _lib.check(L.pf_paged_attn(args, _lib.stream_of(q)), "paged_flash_attention")
+    return restore(o, head_dim, out_dtype)
+
+
+def paged_flash_attention_prefix(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    prefix_table,
+    prefix_len,
+    block_tables,
+    context_lens,
+    *,
+    sm_scale: Optional[float] = None,
+) -> torch.Tensor:
+    """Single-query attention of a batch whose sequences share a prefix
+    (pf_paged_prefix_attn): each sequence attends the prefix's tokens and then
+    its own. The result is that of ``paged_flash_attention`` with the prefix's
+    tokens ahead of every sequence's; the prefix's K/V are read once for the
+    batch instead of once per sequence (the reference's paged call,
+    paged.py:102-192, knows no sharing).
+
+    Args:
+        q: ``[batch, num_heads, 1, head_dim]``.
+        k_pages, v_pages: ``[num_pages, num_kv_heads, page_size, head_dim]``.
+        prefix_table: ``[prefix_pages]`` integer table of the prefix's pages.
+        prefix_len: tokens of the prefix: an int in ``[0, prefix_pages *
+            page_size]`` (its last page need not be full), or a one-entry
+            integer tensor on the device, which is not read back (the call stays
+            capturable) and counts up to the table's reach.
+        block_tables, context_lens: the sequences' own pages and tokens as
+            ``paged_flash_attention`` takes them, the prefix not counted. A
+            sequence without tokens at all yields zeros.
+        sm_scale: default ``1 / sqrt(head_dim)``.
+
+    Returns:
+        ``[batch, num_heads, 1, head_dim]`` in q's dtype. Head dims and dtypes as
+        ``paged_flash_attention``.
+    """
+    if q.dim() != 4 or q.shape[2] != 1:
+        raise ValueError(
+            f"paged attention expects q of shape [batch, heads, 1, head_dim], got {tuple(q.shape)}")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be [num_pages, num_kv_heads, page_size, head_dim] of one shape")
+    batch, num_heads, _, head_dim = q.shape
+    num_pages, num_kv_heads, page_size, k_head_dim = k_pages.shape
+    if k_head_dim != head_dim or num_pages == 0 or page_size == 0:
+        raise ValueError(f"q {tuple(q.shape)} does not match the pool {tuple(k_pages.shape)}")
+    if num_kv_heads == 0 or num_heads == 0 or num_heads % num_kv_heads != 0:
+        raise ValueError(f"num_heads ({num_heads}) must be a multiple of num_kv_heads ({num_kv_heads})")
+    prefix_table, block_tables, context_lens = (torch.as_tensor(t) for t in (prefix_table, block_tables, context_lens))
+    if prefix_table.dim() != 1:
+        raise ValueError(f"prefix_table must be [prefix_pages], got {tuple(prefix_table.shape)}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != batch:
+        raise ValueError(f"block_tables must be [batch, pages_per_seq], got {tuple(block_tables.shape)}")
+    if tuple(context_lens.shape) != (batch,):
+        raise ValueError(f"context_lens must be [batch], got {tuple(context_lens.shape)}")
+    for name, t in (("prefix_table", prefix_table), ("block_tables", block_tables), ("context_lens", context_lens)):
+        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+            raise ValueError(f"{name} must hold integers, got {t.dtype}")
+    reach = prefix_table.shape[0] * page_size
+    on_device = isinstance(prefix_len, torch.Tensor) and prefix_len.device.type != "cpu"
+    if on_device:
+        if prefix_len.numel() != 1 or prefix_len.dtype.is_floating_point or prefix_len.dtype == torch.bool:
+            raise ValueError(f"prefix_len must be one integer, got {tuple(prefix_len.shape)} {prefix_len.dtype}")
+    else:
+        prefix_len = operator.index(prefix_len)
+        if not 0 <= prefix_len <= reach:
+            raise ValueError(f"prefix_len must be in [0, {reach}], got {prefix_len}")
+    if sm_scale is None:
+        sm_scale = 1.0 / (head_dim ** 0.5)
+    _lib.require_device(q, k_pages, v_pages)
+    dev = q.device
+    prefix_table, tables, lens = (t.to(device=dev, dtype=torch.int32).contiguous()
+                                  for t in (prefix_table, block_tables, context_lens))
+    len_t = prefix_len.to(device=dev, dtype=torch.int32).reshape(1) if on_device else None
+    out_dtype = q.dtype
+    cdt = compute_dtype(q, k_pages, v_pages)
+    dp = decode_head_dim(head_dim, cdt)
+    if dp != head_dim or k_pages.dtype != cdt or v_pages.dtype != cdt:
+        warn_copy("paged_flash_attention_prefix", f"head_dim {head_dim} / dtypes {q.dtype}, {k_pages.dtype}, "
+                  f"{v_pages.dtype} are not read in place")
+    q, k_pages, v_pages = (adapt(x.detach(), cdt, dp).contiguous() for x in (q, k_pages, v_pages))
+    o = torch.empty_like(q)
+    if batch == 0:
+        return restore(o, head_dim, out_dtype)
+    args = _lib.PagedPrefixArgs(
+        _lib.ptr(q), _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(prefix_table), _lib.ptr(len_t), _lib.ptr(tables),
+        _lib.ptr(lens), _lib.ptr(o), batch, num_heads, num_kv_heads, num_pages, page_size, dp, prefix_table.shape[0],
+        reach if on_device else prefix_len, tables.shape[1], float(sm_scale), _lib.dtype_tag(q), None, 0)
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        ws_bytes = L.pf_paged_prefix_attn_workspace_size(args)
+        ws = torch.empty(max(int(ws_bytes), 1), dtype=torch.uint8, device=dev)
+        args.workspace = ws.data_ptr()
+        args.workspace_bytes = ws.numel()
+        _lib.check(L.pf_paged_prefix_attn(args, _lib.stream_of(q)), "paged_flash_attention_prefix")
     return restore(o, head_dim, out_dtype)
 
 
@@ -280,4 +377,5 @@ def write_to_paged_cache_rope(
     return q_rot, k_pages, v_pages
 
 
-__all__ = ["paged_flash_attention", "init_paged_cache", "write_to_paged_cache", "write_to_paged_cache_rope"]
+__all__ = ["paged_flash_attention", "paged_flash_attention_prefix", "init_paged_cache", "write_to_paged_cache",
+           "write_to_paged_cache_rope"]
