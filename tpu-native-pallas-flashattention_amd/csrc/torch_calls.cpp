@@ -30,6 +30,9 @@
 #include <cstring>
 #include <exception>
 #include <initializer_list>
+#include <optional>
+#include <utility>
+#include <vector>
 
 #include "../../include/pallas_flash_amd.h"
 
@@ -441,8 +444,295 @@ PyObject* step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// Multi-axis rotation, rotating paged write, shared-prefix attention
+// ---------------------------------------------------------------------------
+// None or a tuple or list of 1 to PF_MAX_ROPE_AXES positive ints that add up to
+// half (None: one axis).
+bool get_sections(PyObject* o, int64_t half, int32_t* axes, int32_t* sections) {
+  if (half < 1 || half > INT_MAX) return false;
+  if (o == Py_None) {
+    *axes = 1;
+    sections[0] = (int32_t)half;
+    return true;
+  }
+  if (!PyTuple_CheckExact(o) && !PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  if (n < 1 || n > PF_MAX_ROPE_AXES) return false;
+  int64_t sum = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!get_len(PySequence_Fast_GET_ITEM(o, i), half, &sections[i])) return false;
+    sum += sections[i];
+  }
+  *axes = (int32_t)n;
+  return sum == half;
+}
+
+// Rotary positions [axes, seq], [axes, batch, seq] (one axis: [seq], [batch,
+// seq]) in device memory, int32 or int64: strides of axis, batch and sequence.
+bool axis_positions(const Tensor* t, const Tensor& q, int32_t axes, int64_t* stride, int32_t* i64) {
+  if (!t || t->device() != q.device() || (t->scalar_type() != at::kInt && t->scalar_type() != at::kLong)) return false;
+  const int64_t batch = q.size(0), seq = q.size(2);
+  int64_t d = t->dim();
+  if (d < 1 || d > 3 || t->size(d - 1) != seq) return false;
+  stride[0] = stride[1] = 0;
+  stride[2] = t->stride(d - 1);
+  if (d == 3) {
+    if (t->size(0) != axes || (t->size(1) != 1 && t->size(1) != batch)) return false;
+    stride[0] = t->stride(0);
+    stride[1] = t->size(1) > 1 ? t->stride(1) : 0;
+  } else if (d == 2 && axes == 1) {
+    if (t->size(0) != 1 && t->size(0) != batch) return false;
+    stride[1] = t->size(0) > 1 ? t->stride(0) : 0;
+  } else if (d == 2) {
+    if (t->size(0) != axes) return false;
+    stride[0] = t->stride(0);
+  } else if (axes != 1) {
+    return false;
+  }
+  *i64 = t->scalar_type() == at::kLong;
+  return true;
+}
+
+bool dense_rows(const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1; }
+
+void set_strides(const Tensor& t, int64_t* stride) {
+  for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+}
+
+// pf_rope_axes of q and k (k may be undefined) into new tensors. `a` holds the
+// positions' and the tables' part.
+std::vector<Tensor> rotate(const Tensor& q, const Tensor& k, pf_rope_axes_args a, bool inverse) {
+  const c10::DeviceGuard guard(q.device());
+  const Tensor q1 = dense_rows(q) ? q : q.contiguous();
+  const Tensor k1 = !k.defined() || dense_rows(k) ? k : k.contiguous();
+  std::vector<Tensor> out{at::empty(q1.sizes(), q1.options())};
+  a.q = q1.data_ptr();
+  a.q_out = out[0].data_ptr();
+  set_strides(q1, a.q_stride);
+  a.num_heads = (int32_t)q1.size(1);
+  a.k = a.k_out = nullptr;
+  a.num_kv_heads = 0;
+  if (k1.defined()) {
+    out.push_back(at::empty(k1.sizes(), k1.options()));
+    a.k = k1.data_ptr();
+    a.k_out = out[1].data_ptr();
+    set_strides(k1, a.k_stride);
+    a.num_kv_heads = (int32_t)k1.size(1);
+  }
+  a.batch = (int32_t)q1.size(0);
+  a.seq_len = (int32_t)q1.size(2);
+  a.head_dim = (int32_t)q1.size(3);
+  a.inverse = inverse ? 1 : 0;
+  a.dtype = dtype_tag(q1);
+  const int st = pf_rope_axes(&a, stream_of(q1));
+  TORCH_CHECK_VALUE(st != PF_ERR_INVALID, "apply_rope_axes: invalid arguments (rejected by the C ABI)");
+  TORCH_CHECK(st == PF_OK, "apply_rope_axes: HIP launch failed (status ", st, ")");
+  return out;
+}
+
+// The rotation is linear: its backward is the transposed rotation, itself
+// differentiable. sections: the axes' pairs.
+struct RopeAxesFn : torch::autograd::Function<RopeAxesFn> {
+  static pf_rope_axes_args args_of(const Tensor& q, const Tensor& positions, const Tensor& cos, const Tensor& sin,
+                                   const std::vector<int64_t>& sections) {
+    pf_rope_axes_args a{};
+    a.axes = (int32_t)sections.size();
+    for (size_t i = 0; i < sections.size(); ++i) a.sections[i] = (int32_t)sections[i];
+    axis_positions(&positions, q, a.axes, a.positions_stride, &a.positions_i64);
+    a.positions = positions.data_ptr();
+    a.cos = cos.data_ptr<float>();
+    a.sin = sin.data_ptr<float>();
+    a.rope_len = (int32_t)cos.size(0);
+    return a;
+  }
+
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q,
+                                                const std::optional<Tensor>& k, const Tensor& positions,
+                                                const Tensor& cos, const Tensor& sin, std::vector<int64_t> sections,
+                                                bool inverse) {
+    ctx->save_for_backward({positions, cos, sin});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["has_k"] = k.has_value();
+    ctx->set_materialize_grads(false);
+    return rotate(q, k.value_or(Tensor()), args_of(q, positions, cos, sin, sections), inverse);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const std::vector<int64_t> sections = ctx->saved_data["sections"].toIntVector();
+    const bool inverse = !ctx->saved_data["inverse"].toBool();
+    Tensor dq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), dk;
+    if (ctx->saved_data["has_k"].toBool() && ctx->needs_input_grad(1)) dk = grads[1];
+    torch::autograd::variable_list out(7);
+    const bool swapped = !dq.defined();
+    if (swapped) std::swap(dq, dk);
+    if (!dq.defined()) return out;
+    auto r = at::GradMode::is_enabled()
+                 ? apply(dq, optional(dk), saved[0], saved[1], saved[2], sections, inverse)
+                 : rotate(dq, dk, args_of(dq, saved[0], saved[1], saved[2], sections), inverse);
+    out[swapped ? 1 : 0] = r[0];
+    if (r.size() > 1) out[1] = r[1];
+    return out;
+  }
+
+  static std::optional<Tensor> optional(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+};
+
+// A [rows, dim] pair of float32 tables.
+bool tables_ok(const Tensor* cos, const Tensor* sin, const Tensor& q) {
+  return cos && sin && cos->dim() == 2 && fits_i32(*cos) && table_ok(cos, q, cos->size(0)) &&
+         table_ok(sin, q, cos->size(0));
+}
+
+// rope_axes(q, k | None, positions, cos, sin, sections) -> (q_rot, k_rot | None) | None
+PyObject* rope_axes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || !plain_thread()) Py_RETURN_NONE;
+  const bool has_k = args[1] != Py_None;
+  const Tensor *q = plain_tensor(args[0]), *k = has_k ? plain_tensor(args[1]) : nullptr;
+  const Tensor *pos = plain_tensor(args[2]), *cos = plain_tensor(args[3]), *sin = plain_tensor(args[4]);
+  pf_rope_axes_args a{};
+  if (!q || (has_k && !k) || !pos || dtype_tag(*q) < 0 || q->dim() != 4 || !fits_i32(*q) || q->size(3) % 2 != 0 ||
+      !dense_rows(*q) || has_tangent({q}))
+    Py_RETURN_NONE;
+  if (has_k && (!same_kind(*q, {k}) || k->dim() != 4 || !fits_i32(*k) || k->size(0) != q->size(0) ||
+                k->size(2) != q->size(2) || k->size(3) != q->size(3) || !dense_rows(*k) || has_tangent({k})))
+    Py_RETURN_NONE;
+  if (!tables_ok(cos, sin, *q) || !get_sections(args[5], q->size(3) / 2, &a.axes, a.sections) ||
+      !axis_positions(pos, *q, a.axes, a.positions_stride, &a.positions_i64))
+    Py_RETURN_NONE;
+  HANDLE_TH_ERRORS
+  std::vector<Tensor> out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const Tensor k1 = has_k ? *k : Tensor();
+    if (wants_grad({q}) || (has_k && wants_grad({k}))) {
+      out = RopeAxesFn::apply(*q, RopeAxesFn::optional(k1), *pos, *cos, *sin, std::vector<int64_t>(a.sections, a.sections + a.axes), false);
+    } else {
+      a.positions = pos->data_ptr();
+      a.cos = cos->data_ptr<float>();
+      a.sin = sin->data_ptr<float>();
+      a.rope_len = (int32_t)cos->size(0);
+      out = rotate(*q, k1, a, false);
+    }
+  }
+  PyObject* both = PyTuple_New(2);
+  if (both == nullptr) return nullptr;
+  for (int i = 0; i < 2; ++i) {
+    PyObject* t = i == 0 || has_k ? THPVariable_Wrap(std::move(out[i])) : Py_NewRef(Py_None);
+    if (t == nullptr) {
+      Py_DECREF(both);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(both, i, t);
+  }
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// rope_write(k_pages, v_pages, q, k, v, block_table, position, cos, sin, rope_positions | None, sections,
+// seq_lens | None) -> q_rot | None (the pools are written in place)
+PyObject* rope_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 12 || !plain_thread()) Py_RETURN_NONE;
+  const Tensor *kp = plain_tensor(args[0]), *vp = plain_tensor(args[1]), *q = plain_tensor(args[2]);
+  const Tensor *k = plain_tensor(args[3]), *v = plain_tensor(args[4]), *tab = plain_tensor(args[5]);
+  const Tensor *pos = plain_tensor(args[6]), *cos = plain_tensor(args[7]), *sin = plain_tensor(args[8]);
+  const bool has_rope = args[9] != Py_None, has_lens = args[11] != Py_None;
+  const Tensor *rope = has_rope ? plain_tensor(args[9]) : nullptr, *lens = has_lens ? plain_tensor(args[11]) : nullptr;
+  pf_rope_paged_write_args a{};
+  if (!kp || !vp || !q || !k || !v || dtype_tag(*q) < 0 || !same_kind(*q, {kp, vp, k, v}) || q->dim() != 4 ||
+      k->dim() != 4 || kp->dim() != 4 || !fits_i32(*q) || !fits_i32(*k) || !fits_i32(*kp) ||
+      kp->sizes() != vp->sizes() || k->sizes() != v->sizes() || !kp->is_contiguous() || !vp->is_contiguous())
+    Py_RETURN_NONE;
+  if (k->size(1) != kp->size(1) || k->size(3) != kp->size(3) || q->size(3) != k->size(3) || q->size(0) != k->size(0) ||
+      q->size(2) != k->size(2) || q->size(1) % k->size(1) != 0 || q->size(3) % 2 != 0 || !dense_rows(*q) ||
+      !dense_rows(*k) || !dense_rows(*v) || has_tangent({kp, vp, q, k, v}))
+    Py_RETURN_NONE;
+  if (!ints_ok(tab, *q) || tab->dim() != 2 || tab->size(0) != q->size(0) || !fits_i32(*tab) || !ints_ok(pos, *q) ||
+      pos->dim() > 1 || (pos->numel() != 1 && pos->numel() != q->size(0)) || !tables_ok(cos, sin, *q) ||
+      !get_sections(args[10], q->size(3) / 2, &a.axes, a.sections))
+    Py_RETURN_NONE;
+  if (has_rope ? !axis_positions(rope, *q, a.axes, a.rope_positions_stride, &a.rope_positions_i64) : a.axes != 1)
+    Py_RETURN_NONE;
+  if (has_lens && (!ints_ok(lens, *q) || lens->dim() != 1 || lens->size(0) != q->size(0))) Py_RETURN_NONE;
+  return guarded([&]() -> Tensor {
+    const c10::DeviceGuard guard(q->device());
+    Tensor out = at::empty(q->sizes(), q->options());
+    a.q = q->data_ptr();
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.q_out = out.data_ptr();
+    a.k_pages = kp->data_ptr();
+    a.v_pages = vp->data_ptr();
+    set_strides(*q, a.q_stride);
+    set_strides(*k, a.k_stride);
+    set_strides(*v, a.v_stride);
+    a.block_tables = tab->data_ptr<int32_t>();
+    a.positions = pos->data_ptr<int32_t>();
+    a.positions_stride = pos->numel() == 1 ? 0 : 1;
+    a.seq_lens = has_lens ? lens->data_ptr<int32_t>() : nullptr;
+    a.rope_positions = has_rope ? rope->data_ptr() : nullptr;
+    a.cos = cos->data_ptr<float>();
+    a.sin = sin->data_ptr<float>();
+    a.rope_len = (int32_t)cos->size(0);
+    a.batch = (int32_t)q->size(0);
+    a.num_heads = (int32_t)q->size(1);
+    a.num_kv_heads = (int32_t)k->size(1);
+    a.seq_len = (int32_t)q->size(2);
+    a.num_pages = (int32_t)kp->size(0);
+    a.page_size = (int32_t)kp->size(2);
+    a.head_dim = (int32_t)q->size(3);
+    a.pages_per_seq = (int32_t)tab->size(1);
+    a.dtype = dtype_tag(*q);
+    accept(pf_rope_paged_cache_write(&a, stream_of(*q)));
+    return out;
+  });
+}
+
+// prefix(q, k_pages, v_pages, prefix_table, prefix_len, block_tables, context_lens, sm_scale) -> o | None
+PyObject* prefix(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8 || !plain_thread()) Py_RETURN_NONE;
+  const Tensor *q = plain_tensor(args[0]), *k = plain_tensor(args[1]), *v = plain_tensor(args[2]);
+  const Tensor *pre = plain_tensor(args[3]), *tab = plain_tensor(args[5]), *lens = plain_tensor(args[6]);
+  float scale;
+  if (!q || !k || !v || !query_ok(*q, *k, *v) || !k->is_contiguous() || !v->is_contiguous() || !ints_ok(pre, *q) ||
+      pre->dim() != 1 || !fits_i32(*pre) || !ints_ok(tab, *q) || tab->dim() != 2 || tab->size(0) != q->size(0) ||
+      !fits_i32(*tab) || !ints_ok(lens, *q) || lens->dim() != 1 || lens->size(0) != q->size(0) ||
+      !get_scale(args[7], q->size(3), &scale))
+    Py_RETURN_NONE;
+  const int64_t reach = pre->size(0) * k->size(2);
+  const Tensor* len = nullptr;
+  int32_t len_host = 0;
+  if (reach > INT_MAX) Py_RETURN_NONE;
+  if (!get_len(args[4], reach, &len_host)) {
+    len = plain_tensor(args[4]);
+    if (!ints_ok(len, *q) || len->numel() != 1) Py_RETURN_NONE;
+    len_host = (int32_t)reach;
+  }
+  return guarded([&]() -> Tensor {
+    const c10::DeviceGuard guard(q->device());
+    const Tensor q1 = q->detach().contiguous();
+    Tensor o = at::empty(q1.sizes(), q1.options());
+    pf_paged_prefix_attn_args a{q1.data_ptr(), k->data_ptr(), v->data_ptr(), pre->data_ptr<int32_t>(),
+                                len != nullptr ? len->data_ptr<int32_t>() : nullptr, tab->data_ptr<int32_t>(),
+                                lens->data_ptr<int32_t>(), o.data_ptr(), (int32_t)q1.size(0), (int32_t)q1.size(1),
+                                (int32_t)k->size(1), (int32_t)k->size(0), (int32_t)k->size(2), (int32_t)q1.size(3),
+                                (int32_t)pre->size(0), len_host, (int32_t)tab->size(1), scale, dtype_tag(q1), nullptr,
+                                0};
+    a.workspace_bytes = pf_paged_prefix_attn_workspace_size(&a);
+    if (a.workspace_bytes == 0) throw Declined();
+    const Tensor ws = bytes(a.workspace_bytes, q1);
+    a.workspace = ws.data_ptr();
+    accept(pf_paged_prefix_attn(&a, stream_of(q1)));
+    return o;
+  });
+}
+
 #define PF_CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {PF_CALL(attention), PF_CALL(rope), PF_CALL(decode), PF_CALL(paged), PF_CALL(step),
+                         PF_CALL(rope_axes), PF_CALL(rope_write), PF_CALL(prefix),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods};
 

@@ -219,7 +219,7 @@ def lib() -> ctypes.CDLL:
 class _Declining:
     """Stands in for _torch_calls: declines every call."""
 
-    attention = rope = decode = paged = step = staticmethod(lambda *args: None)
+    attention = rope = decode = paged = step = rope_axes = rope_write = prefix = staticmethod(lambda *args: None)
 
 
 _calls = None

@@ -146,6 +146,9 @@ def paged_flash_attention_prefix(
         ``[batch, num_heads, 1, head_dim]`` in q's dtype. Head dims and dtypes as
         ``paged_flash_attention``.
     """
+    o = _lib.calls().prefix(q, k_pages, v_pages, prefix_table, prefix_len, block_tables, context_lens, sm_scale)
+    if o is not None:
+        return o
     if q.dim() != 4 or q.shape[2] != 1:
         raise ValueError(
             f"paged attention expects q of shape [batch, heads, 1, head_dim], got {tuple(q.shape)}")
@@ -317,6 +320,10 @@ def write_to_paged_cache_rope(
     Returns ``(q_rot, k_pages, v_pages)``: the rotated q, dense, and the pools.
     No gradients: the pools belong to inference.
     """
+    q_rot = _lib.calls().rope_write(k_pages, v_pages, q, k, v, block_table, position, cos, sin, rope_positions,
+                                    sections, seq_lens)
+    if q_rot is not None:
+        return q_rot, k_pages, v_pages
     from .cache import _check_positions, _positions
     from .rope_axes import (check_axis_positions, check_sections, check_tables, device_positions, rows_of, sections4,
                             strides3)

@@ -155,6 +155,9 @@ def apply_rope_axes(
         ``(q_rot, k_rot)``, dense, in q's dtype; ``k_rot`` is ``None`` without
         k. Differentiable in q and k.
     """
+    out = _lib.calls().rope_axes(q, k, positions, cos, sin, sections)
+    if out is not None:
+        return out
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be rank-4 [batch, heads, seq, head_dim] arrays")
     batch, _, seq, head_dim = q.shape
