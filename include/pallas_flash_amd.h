@@ -338,8 +338,8 @@ int pf_paged_attn_noalloc(const pf_paged_attn_args* args, void* stream);
  * pf_paged_attn.
  * workspace: at least pf_paged_prefix_attn_workspace_size(args) bytes, 256-byte
  * aligned device memory (contents on entry do not matter). The size depends on
- * the shapes, prefix_len and the alignment of q, k_pages and v_pages, not on
- * what the device holds; 0: the call would be refused.
+ * the shapes and prefix_len, not on pointers or what the device holds; 0: the
+ * call would be refused.
  * ------------------------------------------------------------------------- */
 typedef struct {
   const void* q;

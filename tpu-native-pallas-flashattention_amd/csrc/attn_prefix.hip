@@ -4,27 +4,27 @@
 //   o_b = softmax(scale q_b [K_prefix; K_b]^T) [V_prefix; V_b]
 //
 // A paged decode reads the prefix once per sequence. Here the B g query rows
-// of a KV head (all sequences, g heads each) are one matrix against it:
-//  * pf_prefix_kernel: rows x prefix keys on 32x32 MFMAs, one workgroup per
-//    (128 rows, KV head, chunk of keys), leaving (max, sum, acc) of each row
-//    and chunk in float32.
-//  * the sequences' own pages: the paged decode's kernel (decode_stream.hpp;
-//    decode.hip for the forms that does not take), told to leave every
-//    sequence's (max, sum, acc) as well (DecodeParams::partial).
+// of a KV head (all sequences, g heads each) are one matrix against it. Two
+// launches:
+//  * pf_prefix_kernel: one workgroup per work item. A prefix item is 128 rows
+//    of a KV head against one chunk of the prefix's keys; an own item is the g
+//    rows of one sequence and KV head against one chunk of the sequence's keys.
+//    Each leaves (max, sum, acc) of its rows in float32. The prefix items come
+//    first: they are bound by the matrix cores where there are many sequences,
+//    the own items by memory, and both kinds then run beside each other.
 //  * pf_prefix_merge_kernel: o = sum_i acc_i 2^(m_i - M) / sum_i l_i 2^(m_i - M)
-//    over both.
+//    over a row's chunks.
 // No counterpart in the reference, whose paged call gives the prefix's pages
 // to every sequence's table (paged.py:102-192).
 //
-// The prefix kernel is the prefill forward's pipeline (attn_fwd.hip) over pages:
-// K one 64-key block ahead of V, both double-buffered in LDS; S^T = K Q^T runs
-// beside the exponentials of the block before, O^T += V^T P^T beside the
-// maximum of the block after. Its tiles come by direct global -> LDS loads of
-// whole rows (1 KB each, inside one page; rows past the length and columns past
-// the stored head dim lie outside the load's buffer range and arrive as zeros).
-// The pages' first rows are looked up once, into LDS. Pages that such loads
-// would straddle and unaligned pools are staged through registers instead.
-#include "decode_stream.hpp"
+// An item runs the prefill forward's pipeline (attn_fwd.hip) over pages: K one
+// 64-key block ahead of V, both double-buffered in LDS; S^T = K Q^T runs beside
+// the exponentials of the block before, O^T += V^T P^T beside the maximum of the
+// block after. The tiles come by direct global -> LDS loads of whole rows (1 KB
+// each, inside one page; rows past the length and columns past the stored head
+// dim lie outside the load's buffer range and arrive as zeros). The pages' first
+// rows are looked up once, into LDS. Pages that such loads would straddle and
+// unaligned pools are staged through registers instead.
 #include "pf_common.hpp"
 #include "pf_kernels.hpp"
 #include "pf_tiles.hpp"
@@ -36,12 +36,20 @@ namespace {
 constexpr int kBN = 64;      // keys per block
 constexpr int kRows = kPrefixRows;
 
-__device__ inline int prefix_len(const PrefixParams& p) {
-  return p.len_ptr != nullptr ? min(max(stream::sload_i32(p.len_ptr, 0), 0), p.len) : p.len;
+// Scalar load of a wave-uniform address.
+__device__ inline int sload(const int32_t* a) {
+  const __attribute__((address_space(4))) int32_t* c = (const __attribute__((address_space(4))) int32_t*)a;
+  return __builtin_amdgcn_readfirstlane(*c);
 }
+// Keys of the prefix, and of sequence b on its own.
+__device__ inline int prefix_len(const PrefixParams& p) {
+  return p.len_ptr != nullptr ? min(max(sload(p.len_ptr), 0), p.len) : p.len;
+}
+__device__ inline int own_len(const PrefixParams& p, int b) { return min(max(sload(p.own_lens + b), 0), p.own_cap); }
 
-// Loads of 64-row tiles of a pool. DMA: each wave's loads are RPL whole rows of
-// one page; else every lane fetches its 16-byte chunks itself.
+// Loads of 64-row tiles of keys [key0, key0 + kv_len) of a table's pages. DMA:
+// each wave's loads are RPL whole rows of one page; else every lane fetches its
+// 16-byte chunks itself.
 template <typename T, int D, bool DMA>
 struct PageTiles {
   using G = Tile<T, D>;
@@ -50,16 +58,18 @@ struct PageTiles {
   uint32_t voff[PT];  // DMA: the lane's byte offset within the load's rows
   uint32_t row0;      // DMA: the wave's first row of load 0; load u: + 4 RPL u
   uint32_t slot0;     // the wave's LDS byte offset of load 0; load u: + 4096 u
-  int lane, kv_len, last;
+  int lane, kv_len, last, key0, kvh;
   const PrefixParams& p;
-  const uint32_t* first;  // LDS: row number (in rows of the pool) of each group of keys
+  const int32_t* table;
+  const uint32_t* first;  // LDS: pool row of each group of keys
 
-  __device__ inline PageTiles(const PrefixParams& p_, int tid, int kv_len_, const uint32_t* first_)
-      : lane(tid & 63), kv_len(kv_len_), p(p_), first(first_) {
+  // groups: of keys looked up, at least 1
+  __device__ inline PageTiles(const PrefixParams& p_, int tid, int key0_, int kv_len_, int groups, int kvh_,
+                              const int32_t* table_, const uint32_t* first_)
+      : lane(tid & 63), kv_len(kv_len_), last(groups - 1), key0(key0_), kvh(kvh_), p(p_), table(table_), first(first_) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     row0 = RPL * w;
     slot0 = 1024 * w;
-    last = (kv_len - 1) >> p.group_log2;
 #pragma unroll
     for (int u = 0; u < PT; ++u) {
       const int r = lane / G::CPR, row = RPL * (4 * u + w) + r;
@@ -82,7 +92,7 @@ struct PageTiles {
     dma16(d, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 4096 * u));
   }
   // Without DMA: block j through registers.
-  __device__ inline void copy(const void* pool, int kvh, int key0, int j, char* tile) const {
+  __device__ inline void copy(const void* pool, int j, char* tile) const {
     u32x4 x[PT];
 #pragma unroll
     for (int u = 0; u < PT; ++u) {
@@ -91,7 +101,7 @@ struct PageTiles {
       x[u] = (u32x4){0u, 0u, 0u, 0u};
       if (key < kv_len && chunk * G::EPC < p.dr) {
         const int lp = (key0 + key) / p.page_size;
-        const int page = min(max(p.table[lp], 0), p.num_pages - 1);
+        const int page = min(max(table[lp], 0), p.num_pages - 1);
         const int64_t at = ((int64_t)page * p.Hkv + kvh) * p.page_size + (key0 + key - lp * p.page_size);
         x[u] = ldg16(static_cast<const T*>(pool) + at * p.dr + chunk * G::EPC);
       }
@@ -116,26 +126,53 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hh = lane >> 5, l32 = lane & 31;
 
-  // (chunk, kv head, row tile): the row tiles of one chunk side by side on one
-  // XCD, whose L2 then serves the chunk to all of them.
-  const int item = xcd_remap(blockIdx.x, p.n_tiles * p.Hkv * p.n_split, p.n_tiles);
-  const int tile = item % p.n_tiles, kvh = item / p.n_tiles % p.Hkv, split = item / p.n_tiles / p.Hkv;
-  const int len = prefix_len(p);
-  const int key0 = split * p.chunk;
-  if (key0 >= len) return;  // the merge counts the chunks below len
-  const int kv_len = min(len - key0, p.chunk);
-  const int nblk = (kv_len + kBN - 1) / kBN;
-
+  // The item: rows, table, and keys [key0, key0 + chunk) below len.
+  const int32_t* table;
+  int kvh, b0, r0, piece, key0, chunk, cap, len;
+  const bool own = blockIdx.x >= (unsigned)p.n_pre;
+  if (!own) {
+    // (chunk, kv head, row tile): the row tiles of one chunk side by side on one
+    // XCD, whose L2 then serves the chunk to all of them.
+    const int item = xcd_remap(blockIdx.x, p.n_pre, p.n_tiles);
+    r0 = kRows * (item % p.n_tiles);
+    kvh = item / p.n_tiles % p.Hkv;
+    piece = item / p.n_tiles / p.Hkv;
+    b0 = 0;
+    table = p.table;
+    chunk = p.chunk;
+    key0 = piece * chunk;
+    cap = p.len;
+    len = prefix_len(p);
+  } else {
+    // chunk by chunk, so that the items past the sequences' ends come last
+    const int item = blockIdx.x - p.n_pre, seqs = p.B * p.Hkv * p.n_hc;
+    const int c = item / seqs, sq = item - c * seqs;
+    r0 = kRows * (sq % p.n_hc);
+    kvh = sq / p.n_hc % p.Hkv;
+    b0 = sq / p.n_hc / p.Hkv;
+    piece = p.n_split + c;
+    table = p.own_tables + (int64_t)b0 * p.pages_per_seq;
+    chunk = p.own_chunk;
+    key0 = c * chunk;
+    cap = p.own_cap;
+    len = own_len(p, b0);
+  }
+  // The lookups do not wait for the length: entries past it (-1 padding) are
+  // clamped, and no row of theirs is read.
+  const int groups = (min(chunk, cap - key0) + (1 << p.group_log2) - 1) >> p.group_log2;
   if constexpr (DMA) {
-    for (int i = tid; i <= (kv_len - 1) >> p.group_log2; i += 256) {
+    for (int i = tid; i < groups; i += 256) {
       const int key = key0 + (i << p.group_log2);
       const int lp = key / p.page_size;
-      const int page = min(max(p.table[lp], 0), p.num_pages - 1);
+      const int page = min(max(table[lp], 0), p.num_pages - 1);
       first[i] = ((uint32_t)page * p.Hkv + kvh) * p.page_size + (key - lp * p.page_size);
     }
-    __syncthreads();
   }
-  const PTiles tiles(p, tid, kv_len, first);
+  if (key0 >= len) return;  // the merge counts the chunks below len
+  const int kv_len = min(len - key0, chunk);
+  const int nblk = (kv_len + kBN - 1) / kBN;
+  if constexpr (DMA) __syncthreads();
+  const PTiles tiles(p, tid, key0, kv_len, groups, kvh, table, first);
   char* const kbuf0 = smem;
   char* const vbuf0 = smem + 2 * G::BYTES;
   auto whole = [&](const void* pool, int j, char* t) {
@@ -143,24 +180,27 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
 #pragma unroll
       for (int u = 0; u < PT; ++u) tiles.load(pool, tiles.row_of(j, u), j, u, t);
     } else {
-      tiles.copy(pool, kvh, key0, j, t);
+      tiles.copy(pool, j, t);
     }
   };
   whole(p.k, 0, kbuf0);
   whole(p.v, 0, vbuf0);
   if (nblk > 1) whole(p.k, 1, kbuf0 + G::BYTES);
 
-  // Q: the lane's row of the tile, columns [hh HALF, + HALF).
-  const int r = kRows * tile + 32 * wv + l32;
-  const bool active = kRows * tile + 32 * wv < p.rows;  // the wave has rows at all
-  const int b = r / p.g, h = kvh * p.g + (r - b * p.g);
+  // Q: the lane's row, columns [hh HALF, + HALF). An own item seldom has rows for
+  // more than one wave: which one differs from item to item, so that the items
+  // on a CU load all of its SIMDs.
+  const int rw = r0 + 32 * (own ? (wv + blockIdx.x) & 3 : wv), r = rw + l32;
+  const int n_rows = own ? p.g : p.rows;
+  const bool active = rw < n_rows;  // the wave has rows at all
+  const int b = own ? b0 : r / p.g, h = kvh * p.g + (own ? r : r - b * p.g);
   Frag qf[QF];
   {
     const T* qr = static_cast<const T*>(p.q) + ((int64_t)b * p.Hq + h) * p.dr + hh * HALF;
     u32x4 qc[HALF / EPC];
 #pragma unroll
     for (int c = 0; c < HALF / EPC; ++c)
-      qc[c] = r < p.rows && hh * HALF + c * EPC < p.dr ? ldg16(qr + c * EPC) : (u32x4){0u, 0u, 0u, 0u};
+      qc[c] = r < n_rows && hh * HALF + c * EPC < p.dr ? ldg16(qr + c * EPC) : (u32x4){0u, 0u, 0u, 0u};
     if (p.scale_log2 < 0.f) {  // |scale| on -Q
       const uint32_t sign = G::ES == 4 ? 0x80000000u : 0x80008000u;
 #pragma unroll
@@ -241,8 +281,8 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
 #pragma unroll
       for (int u = 0; u < PT; ++u) row_k[u] = tiles.row_of(j + 2, u);
     } else {
-      if (k_next) tiles.copy(p.k, kvh, key0, j + 2, kdst);
-      tiles.copy(p.v, kvh, key0, j + 1, vdst);
+      if (k_next) tiles.copy(p.k, j + 2, kdst);
+      tiles.copy(p.v, j + 1, vdst);
     }
     if (!active) {
 #pragma unroll
@@ -340,65 +380,28 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
     mfma_trn<T, D>(vbuf0 + ((nblk - 1) & 1) * G::BYTES, lane, vta, pfr, acc);
   }
   const float l_tot = wave_xor32_sum(l_run);
-  if (r < p.rows) {
-    const int64_t at = (int64_t)split * p.B * p.Hq + (int64_t)b * p.Hq + h;
+  if (r < n_rows) {
+    const int64_t at = (int64_t)piece * p.B * p.Hq + (int64_t)b * p.Hq + h;
     store_acc_row<float, D>(p.part_o + at * D, acc, 1.f, hh);
     if (hh == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * at) = (f32x2){m_run, l_tot};
   }
 }
 
-// The merge: a workgroup per sequence (batch, kv head, 16-head slice). Its own
-// pieces, by DecodeParams::partial: 1, one slot per sequence; 2, the streaming
-// kernel's pieces, located in its work list by one wave; 0 with n_waves = 0, the
-// generic kernel's chunks; none where the own table is empty. Then the live
-// chunks of the prefix. D / 4 lanes a row, 16 bytes each; where the rows leave
-// lanes over, groups of lanes share the pieces and join through LDS. Bound by
-// the pieces' latency: 8 are in flight per lane.
-template <typename T, int D, bool FINE>
-__global__ __launch_bounds__(256) void pf_prefix_merge_kernel(DecodeParams p, PrefixParams pre) {
-  constexpr int SK = stream::StreamGeo<T, D, FINE>::SK;
-  constexpr int PG = 2;  // paged lengths
+// The merge: a workgroup per (batch, kv head, 16 of its heads), D / 4 lanes a
+// row, 16 bytes each; where the rows leave lanes over, groups of lanes share the
+// chunks and join through LDS. Bound by the partials' latency: 8 are in flight
+// per lane.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
   constexpr int LPR = D / 4, NB = 8;
-  const int g = pre.g, n_hc = (g + 15) >> 4, J = pre.Hkv * n_hc;
+  const int g = p.g, n16 = (g + 15) >> 4, J = p.Hkv * n16;
   const int b = blockIdx.x / J, j = blockIdx.x - b * J;
-  const int kvh = j / n_hc, hc = j - kvh * n_hc;
+  const int kvh = j / n16, hc = j - kvh * n16;
   const int nq = min(16, g - 16 * hc);
-  const int64_t seq = blockIdx.x;
   const int tid = threadIdx.x;
-
-  __shared__ int found[3];  // pieces, first wave, whether it starts inside that wave's range
-  int np = 0, wa = 0;
-  bool late = false;
-  if (p.partial == 2) {
-    if (tid < 64) {
-      const stream::BatchScan sc = stream::batch_scan<PG, SK>(p, J);
-      const stream::Partition part(sc.tot, p.n_waves);
-      const int L = sc.per == 1 ? __builtin_amdgcn_readlane(sc.L, b) : stream::seq_len<PG>(p, b);
-      const int nst = (L + SK - 1) / SK;
-      if (nst > 0) {
-        const int64_t s0 = stream::stages_before<PG, SK>(p, J, b, sc) + (int64_t)j * nst;
-        wa = part.wave_of(s0);
-        np = part.wave_of(s0 + nst - 1) - wa + 1;
-        late = part.start(wa) < s0;
-      }
-      if (tid == 0) {
-        found[0] = np;
-        found[1] = wa;
-        found[2] = late;
-      }
-    }
-    __syncthreads();
-    np = found[0];
-    wa = found[1];
-    late = found[2] != 0;
-  } else if (p.partial == 1) {
-    np = 1;
-  } else if (p.pages_per_seq > 0) {
-    const int L = min(max(p.context_lens[b], 0), p.pages_per_seq * p.page_size);
-    np = (L + p.chunk - 1) / p.chunk;
-  }
-  const int npre = (prefix_len(pre) + pre.chunk - 1) / pre.chunk;
-  const int total = np + npre;
+  // the live chunks: of the prefix, then of the sequence
+  const int npre = (prefix_len(p) + p.chunk - 1) / p.chunk;
+  const int total = npre + (p.n_own > 0 ? (own_len(p, b) + p.own_chunk - 1) / p.own_chunk : 0);
 
   __shared__ f32x4 so[256];
   __shared__ f32x2 sm[256];
@@ -409,8 +412,7 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(DecodeParams p, Pr
     const int i = per >= 256 ? i0 + tid : tid - grp * per;
     const bool on = i < per && grp < ngrp;
     const int qi = on ? i / LPR : 0, d0 = on ? 4 * (i % LPR) : 0;
-    const int h = kvh * g + 16 * hc + qi;
-    const int64_t bh = (int64_t)b * pre.Hq + h;
+    const int64_t bh = (int64_t)b * p.Hq + kvh * g + 16 * hc + qi;
     float M = kNegInf, l = 0.f;
     f32x4 o = (f32x4)(0.f);
     for (int c0 = grp; on && c0 < total; c0 += NB * ngrp) {
@@ -423,23 +425,9 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(DecodeParams p, Pr
         ml[c] = (f32x2){kNegInf, 0.f};
         v[c] = (f32x4)(0.f);
         if (s < total) {
-          const float* po = p.part_o;
-          const float* pm = p.part_ml;
-          int64_t row;
-          if (s >= np) {
-            po = pre.part_o;
-            pm = pre.part_ml;
-            row = (int64_t)(s - np) * pre.B * pre.Hq + bh;
-          } else if (p.partial == 2) {
-            row = (np == 1 ? stream::whole_slot(p, J, wa, seq) : stream::piece_slot(p, J, wa + s, seq, s == 0 && late)) *
-                      p.qrows + qi;
-          } else if (p.partial == 1) {
-            row = seq * p.qrows + qi;
-          } else {
-            row = bh * p.n_split + s;
-          }
-          ml[c] = *reinterpret_cast<const f32x2*>(pm + row * 2);
-          v[c] = *reinterpret_cast<const f32x4*>(po + row * D + d0);
+          const int64_t row = (int64_t)(s < npre ? s : p.n_split + s - npre) * p.B * p.Hq + bh;
+          ml[c] = *reinterpret_cast<const f32x2*>(p.part_ml + row * 2);
+          v[c] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + d0);
         }
         Mn = fmaxf(Mn, ml[c][0]);
       }
@@ -462,9 +450,9 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(DecodeParams p, Pr
       if (grp != 0) return;
       for (int k = 1; k < ngrp; ++k) M = fmaxf(M, sm[tid + k * per][0]);
       const float Mu = (M == kNegInf) ? 0.f : M;
-      const float own = exp2f(sm[tid][0] - Mu);
-      o *= own;
-      l *= own;
+      const float mine = exp2f(sm[tid][0] - Mu);
+      o *= mine;
+      l *= mine;
       for (int k = 1; k < ngrp; ++k) {
         const f32x2 x = sm[tid + k * per];
         const float wt = exp2f(x[0] - Mu);
@@ -472,63 +460,49 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(DecodeParams p, Pr
         o += so[tid + k * per] * wt;
       }
     }
-    if (on && d0 < pre.dr) {
+    if (on && d0 < p.dr) {
       const float inv = (l == 0.f) ? 0.f : 1.f / l;  // no key, or none that weighs: o = 0
       typedef T v4 __attribute__((ext_vector_type(4)));
       v4 y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f32(o[e] * inv);
-      *reinterpret_cast<v4*>(static_cast<T*>(p.o) + bh * pre.dr + d0) = y;
+      *reinterpret_cast<v4*>(static_cast<T*>(p.o) + bh * p.dr + d0) = y;
     }
   }
 }
 
 template <typename T, int D>
-hipError_t launch_prefix_dim(const PrefixParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.n_tiles * p.Hkv * p.n_split));
-  if (p.dma) hipLaunchKernelGGL((pf_prefix_kernel<T, D, true>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((pf_prefix_kernel<T, D, false>), grid, dim3(256), 0, st, p);
-  return hipGetLastError();
-}
-
-template <typename T, int D>
-hipError_t launch_merge_dim(const DecodeParams& own, const PrefixParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.B * p.Hkv * ((p.g + 15) / 16)));
-  if constexpr (sizeof(T) == 4 && D == 64) {
-    if (own.fine) {
-      hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D, true>), grid, dim3(256), 0, st, own, p);
-      return hipGetLastError();
-    }
+hipError_t launch_typed(const PrefixParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.n_pre + p.n_own * p.B * p.Hkv * p.n_hc));
+  if (grid.x > 0) {
+    if (p.dma) hipLaunchKernelGGL((pf_prefix_kernel<T, D, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((pf_prefix_kernel<T, D, false>), grid, dim3(256), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D, false>), grid, dim3(256), 0, st, own, p);
+  hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D>), dim3((unsigned)(p.B * p.Hkv * ((p.g + 15) / 16))), dim3(256), 0,
+                     st, p);
   return hipGetLastError();
 }
 
-template <typename F>
-hipError_t by_type(int dtype, int D, F&& f) {
-  auto dims = [&](auto t) {
-    using T = decltype(t);
-    if (D == 64) return f(t, std::integral_constant<int, 64>{});
-    if (D == 128) return f(t, std::integral_constant<int, 128>{});
-    if constexpr (sizeof(T) == 2)
-      if (D == 256) return f(t, std::integral_constant<int, 256>{});
-    return hipErrorInvalidValue;
-  };
-  if (dtype == kF32) return dims(float());
-  if (dtype == kBF16) return dims(bf16_t());
-  if (dtype == kF16) return dims(f16_t());
+template <typename T>
+hipError_t launch_dim(const PrefixParams& p, int D, hipStream_t st) {
+  if (D == 64) return launch_typed<T, 64>(p, st);
+  if (D == 128) return launch_typed<T, 128>(p, st);
+  if constexpr (sizeof(T) == 2)
+    if (D == 256) return launch_typed<T, 256>(p, st);
   return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 hipError_t launch_prefix(const PrefixParams& p, int dtype, int D, hipStream_t stream) {
-  return by_type(dtype, D, [&](auto t, auto d) { return launch_prefix_dim<decltype(t), decltype(d)::value>(p, stream); });
-}
-
-hipError_t launch_prefix_merge(const DecodeParams& own, const PrefixParams& p, int dtype, int D, hipStream_t stream) {
-  return by_type(dtype, D,
-                 [&](auto t, auto d) { return launch_merge_dim<decltype(t), decltype(d)::value>(own, p, stream); });
+  switch (dtype) {
+    case kF32: return launch_dim<float>(p, D, stream);
+    case kBF16: return launch_dim<bf16_t>(p, D, stream);
+    case kF16: return launch_dim<f16_t>(p, D, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace pf

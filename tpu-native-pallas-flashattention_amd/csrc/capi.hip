@@ -874,133 +874,102 @@ int pf_paged_attn(const pf_paged_attn_args* a, void* stream) {
 // ---------------------------------------------------------------------------
 namespace {
 
-struct PrefixPlan {
-  pf::PrefixParams pre;
-  pf::DecodeParams own;
-  int D;                // compute head dim
-  size_t pre_rows, own_rows;  // partials
-  size_t bytes() const { return partial_bytes(pre_rows, D) + partial_bytes(own_rows, D); }
-};
-
-// Chunks of the prefix: as many workgroups as are resident at once.
-void plan_prefix_chunks(pf::PrefixParams* p, int32_t dtype, int D) {
-  const int64_t items = (int64_t)p->n_tiles * p->Hkv;
-  const int per_cu = D == 64 && dtype != PF_DTYPE_F32 ? 3 : (D == 256 || (D == 128 && dtype == PF_DTYPE_F32)) ? 1 : 2;
-  const int64_t n = std::max<int64_t>(1, kCus * per_cu / items);
-  int64_t chunk = ((p->len + n - 1) / n + 63) / 64 * 64;
-  if (chunk < 128) chunk = 128;
-  if (p->dma) chunk = std::min<int64_t>(chunk, (int64_t)pf::kPrefixGroups << p->group_log2);
-  p->chunk = (int)chunk;
-  p->n_split = (int)((p->len + chunk - 1) / chunk);
+// The chunks. Prefix: one item per CU; own: enough items to go round, chunks of
+// 128 to 1024 keys.
+void plan_prefix(pf::PrefixParams* p) {
+  const int64_t most = p->dma ? (int64_t)pf::kPrefixGroups << p->group_log2 : (int64_t)1 << 30;
+  auto chunk_of = [&](int64_t keys, int64_t pieces, int64_t lo, int64_t hi) {
+    const int64_t c = ((keys + pieces - 1) / pieces + 63) / 64 * 64;
+    return (int)std::min(most, std::min(hi, std::max(lo, c)));
+  };
+  const int64_t items = (int64_t)p->n_tiles * p->Hkv, seqs = (int64_t)p->B * p->Hkv * p->n_hc;
+  p->chunk = p->own_chunk = 64;
+  if (p->len > 0) {
+    p->chunk = chunk_of(p->len, std::max<int64_t>(1, kCus / items), 128, (int64_t)1 << 30);
+    p->n_split = (p->len + p->chunk - 1) / p->chunk;
+  }
+  if (p->own_cap > 0) {
+    p->own_chunk = chunk_of(p->own_cap, std::max<int64_t>(1, 4 * kCus / seqs), 128, 1024);
+    p->n_own = (p->own_cap + p->own_chunk - 1) / p->own_chunk;
+  }
 }
 
-int fill_prefix(const pf_paged_prefix_attn_args* a, PrefixPlan* plan) {
+// *D: the compute head dim.
+int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D) {
   if (!a) return PF_ERR_INVALID;
-  if (a->prefix_pages < 0 || a->prefix_len < 0 || a->page_size < 1 ||
-      a->prefix_len > (int64_t)a->prefix_pages * a->page_size)
+  if (a->batch < 0 || a->num_heads < 1 || a->num_kv_heads < 1 || a->num_pages < 1 || a->page_size < 1 ||
+      a->pages_per_seq < 0 || a->prefix_pages < 0 || a->prefix_len < 0)
     return PF_ERR_INVALID;
-  // the sequences' own part: a paged decode
-  const pf_paged_attn_args own{a->q, a->k_pages, a->v_pages, a->block_tables, a->context_lens, a->o,
-                               a->batch, a->num_heads, a->num_kv_heads, a->num_pages, a->page_size, a->head_dim,
-                               a->pages_per_seq, a->sm_scale, a->dtype, nullptr, 0};
-  bool streams;
-  pf::DecodeParams& d = plan->own;
-  int st = fill_paged(&own, &d, &streams, SIZE_MAX);
-  if (st != PF_OK) return st;
-  const int D = plan->D = d.D;
-  if (d.n_waves == 0) {  // all batches in one launch
-    st = generic_setup(&d, std::max<int64_t>(1, (int64_t)a->pages_per_seq * a->page_size), 0);
-    if (st != PF_OK) return st;
-  }
-  const int group = a->num_heads / a->num_kv_heads;
-  const int64_t seqs = (int64_t)a->batch * a->num_kv_heads * ((group + 15) / 16);
-  if (seqs > kMaxGrid || (int64_t)a->batch * a->num_heads > kMaxGrid - 2 * pf::kPrefixRows) return PF_ERR_UNSUPPORTED;
-  d.qrows = pf::decode_stream_qrows(group);
-  if (a->pages_per_seq == 0) {
-    plan->own_rows = 0;
-    d.n_waves = d.partial = 0;
-  } else if (d.n_waves == 0) {
-    d.partial = 0;
-    plan->own_rows = (size_t)a->batch * a->num_heads * d.n_split;
-  } else if (pf::decode_stream_short(d, a->dtype, true)) {
-    d.partial = 1;
-    plan->own_rows = (size_t)seqs * d.qrows;
-  } else {
-    d.partial = 2;
-    plan->own_rows = (size_t)(seqs + (seqs <= d.n_waves ? 1 : 2) * (int64_t)d.n_waves) * d.qrows;
-  }
-
-  pf::PrefixParams& p = plan->pre;
-  p = pf::PrefixParams{};
-  p.q = a->q;
-  p.k = a->k_pages;
-  p.v = a->v_pages;
-  p.table = a->prefix_table;
-  p.len_ptr = a->prefix_len_ptr;
-  p.len = a->prefix_len;
-  p.B = a->batch;
-  p.Hq = a->num_heads;
-  p.Hkv = a->num_kv_heads;
-  p.g = group;
-  p.rows = a->batch * group;
-  p.dr = a->head_dim;
-  p.num_pages = a->num_pages;
-  p.page_size = a->page_size;
-  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
-  p.n_tiles = (p.rows + pf::kPrefixRows - 1) / pf::kPrefixRows;
-  const int rows_per_load = 1024 / (D * (a->dtype == PF_DTYPE_F32 ? 4 : 2));
-  while (p.group_log2 < 6 && a->page_size % (2 << p.group_log2) == 0) ++p.group_log2;
+  if (a->num_heads % a->num_kv_heads != 0) return PF_ERR_INVALID;
+  if (a->prefix_len > (int64_t)a->prefix_pages * a->page_size) return PF_ERR_INVALID;
+  if (!isfinite(a->sm_scale)) return PF_ERR_INVALID;
+  if (!dtype_ok(a->dtype)) return PF_ERR_UNSUPPORTED;
+  if (!decode_head_dim_ok(a->head_dim, a->dtype)) return PF_ERR_UNSUPPORTED;
+  *D = decode_compute_dim(a->head_dim);
+  const int64_t own_cap = (int64_t)a->pages_per_seq * a->page_size;
+  if (own_cap > kMaxGrid - 2048 || a->prefix_len > kMaxGrid - 2048) return PF_ERR_UNSUPPORTED;
+  if ((int64_t)a->batch * a->num_heads > kMaxGrid - 2 * pf::kPrefixRows) return PF_ERR_UNSUPPORTED;
+  *p = pf::PrefixParams{};
+  p->q = a->q;
+  p->k = a->k_pages;
+  p->v = a->v_pages;
+  p->o = a->o;
+  p->B = a->batch;
+  p->Hq = a->num_heads;
+  p->Hkv = a->num_kv_heads;
+  p->g = a->num_heads / a->num_kv_heads;
+  p->rows = a->batch * p->g;
+  p->dr = a->head_dim;
+  p->num_pages = a->num_pages;
+  p->page_size = a->page_size;
+  p->scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p->table = a->prefix_table;
+  p->len_ptr = a->prefix_len_ptr;
+  p->len = a->prefix_len;
+  p->n_tiles = (p->rows + pf::kPrefixRows - 1) / pf::kPrefixRows;
+  p->own_tables = a->block_tables;
+  p->own_lens = a->context_lens;
+  p->pages_per_seq = a->pages_per_seq;
+  p->own_cap = (int)own_cap;
+  p->n_hc = (p->g + pf::kPrefixRows - 1) / pf::kPrefixRows;
+  const int rows_per_load = 1024 / (*D * (a->dtype == PF_DTYPE_F32 ? 4 : 2));
+  while (p->group_log2 < 6 && a->page_size % (2 << p->group_log2) == 0) ++p->group_log2;
   // pool rows are counted in 32 bits
-  p.dma = a->page_size % rows_per_load == 0 &&
-          (int64_t)a->num_pages * a->page_size <= (int64_t)0xffffffff / a->num_kv_heads;
-  p.chunk = 64;
-  plan->pre_rows = 0;
-  if (p.len > 0 && a->batch > 0) {
-    plan_prefix_chunks(&p, a->dtype, D);
-    if ((int64_t)p.n_tiles * p.Hkv * p.n_split > kMaxGrid) return PF_ERR_UNSUPPORTED;
-    plan->pre_rows = (size_t)p.n_split * a->batch * a->num_heads;
-  }
-  p.dma = p.dma && (((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0;
+  p->dma = a->page_size % rows_per_load == 0 &&
+           (int64_t)a->num_pages * a->page_size <= (int64_t)0xffffffff / a->num_kv_heads;
+  if (a->batch > 0) plan_prefix(p);
+  const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
+  const int64_t n_own = (int64_t)p->B * p->Hkv * p->n_hc * p->n_own;
+  if (n_pre + n_own > kMaxGrid) return PF_ERR_UNSUPPORTED;
+  p->n_pre = (int)n_pre;
+  p->dma = p->dma && (((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0;
   return PF_OK;
 }
+
+size_t prefix_rows(const pf::PrefixParams& p) { return (size_t)(p.n_split + p.n_own) * p.B * p.Hq; }
+size_t prefix_ws(const pf::PrefixParams& p, int D) { return std::max<size_t>(partial_bytes(prefix_rows(p), D), 256); }
 
 }  // namespace
 
 size_t pf_paged_prefix_attn_workspace_size(const pf_paged_prefix_attn_args* a) {
-  PrefixPlan plan;
-  if (fill_prefix(a, &plan) != PF_OK) return 0;
-  return std::max<size_t>(plan.bytes(), 256);
+  pf::PrefixParams p;
+  int D;
+  return fill_prefix(a, &p, &D) == PF_OK ? prefix_ws(p, D) : 0;
 }
 
 int pf_paged_prefix_attn(const pf_paged_prefix_attn_args* a, void* stream) {
-  PrefixPlan plan;
-  int st = fill_prefix(a, &plan);
+  pf::PrefixParams p;
+  int D;
+  const int st = fill_prefix(a, &p, &D);
   if (st != PF_OK) return st;
   if (a->batch == 0) return PF_OK;
   if (!a->q || !a->k_pages || !a->v_pages || !a->o || !a->context_lens) return PF_ERR_INVALID;
   if ((a->pages_per_seq > 0 && !a->block_tables) || (a->prefix_len > 0 && !a->prefix_table)) return PF_ERR_INVALID;
-  if (!a->workspace || a->workspace_bytes < std::max<size_t>(plan.bytes(), 256) || ((uintptr_t)a->workspace & 255) != 0)
+  if (!a->workspace || a->workspace_bytes < prefix_ws(p, D) || ((uintptr_t)a->workspace & 255) != 0)
     return PF_ERR_WORKSPACE;
-  auto bind = [D = plan.D](char*& ws, size_t rows, float** o, float** ml) {
-    *o = reinterpret_cast<float*>(ws);
-    *ml = reinterpret_cast<float*>(ws + align256(rows * D * sizeof(float)));
-    ws += partial_bytes(rows, D);
-  };
-  char* ws = static_cast<char*>(a->workspace);
-  bind(ws, plan.pre_rows, &plan.pre.part_o, &plan.pre.part_ml);
-  bind(ws, plan.own_rows, &plan.own.part_o, &plan.own.part_ml);
-  hipStream_t s = (hipStream_t)stream;
-  if (plan.pre_rows > 0) {
-    st = finish(pf::launch_prefix(plan.pre, a->dtype, plan.D, s));
-    if (st != PF_OK) return st;
-  }
-  if (plan.own_rows > 0) {
-    pf::DecodeParams d = plan.own;
-    if (d.n_waves == 0) d.partial = 2;  // the generic kernel: no combine of its own
-    st = finish(pf::launch_decode(d, a->dtype, true, s));
-    if (st != PF_OK) return st;
-  }
-  return finish(pf::launch_prefix_merge(plan.own, plan.pre, a->dtype, plan.D, s));
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + align256(prefix_rows(p) * D * sizeof(float)));
+  return finish(pf::launch_prefix(p, a->dtype, D, (hipStream_t)stream));
 }
 
 }  // extern "C"

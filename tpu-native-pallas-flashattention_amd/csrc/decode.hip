@@ -367,7 +367,7 @@ hipError_t launch_decode_combine(const DecodeParams& p, int dtype, bool paged, h
 hipError_t launch_decode(const DecodeParams& p, int dtype, bool paged, hipStream_t stream) {
   if (p.n_waves > 0) return launch_decode_stream(p, dtype, paged, stream);
   hipError_t e = paged ? launch_dtype<true>(p, dtype, false, stream) : launch_dtype<false>(p, dtype, false, stream);
-  if (e != hipSuccess || p.partial != 0) return e;
+  if (e != hipSuccess) return e;
   return launch_decode_combine(p, dtype, paged, stream);
 }
 

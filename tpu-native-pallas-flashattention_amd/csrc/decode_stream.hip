@@ -94,21 +94,6 @@ int decode_stream_waves(int dtype, int head_dim, int stages, int group, bool fin
   return cus * (per_cu > 1 ? per_cu : 1);
 }
 
-bool decode_stream_short(const DecodeParams& p, int dtype, bool paged) {
-  const bool small = decode_stream_qrows(p.Hq / p.Hkv) == 4, f32 = dtype == kF32;
-  auto fits = [&](auto t, auto d) {
-    using T = decltype(t);
-    constexpr int D = decltype(d)::value;
-    return small ? stream::short_form<T, D, 4>(p, paged) : stream::short_form<T, D, 16>(p, paged);
-  };
-  using I64 = std::integral_constant<int, 64>;
-  using I128 = std::integral_constant<int, 128>;
-  using I256 = std::integral_constant<int, 256>;
-  if (p.D == 64) return f32 ? fits(float(), I64{}) : fits(bf16_t(), I64{});
-  if (p.D == 128) return f32 ? fits(float(), I128{}) : fits(bf16_t(), I128{});
-  return fits(bf16_t(), I256{});
-}
-
 int decode_stream_qrows(int group) { return group <= 4 ? 4 : 16; }
 
 hipError_t launch_decode_stream(const DecodeParams& p, int dtype, bool paged, hipStream_t stream) {

@@ -247,12 +247,6 @@ __device__ inline int64_t piece_slot(const DecodeParams& p, int J, int w, int64_
   return (int64_t)p.B * J <= p.n_waves ? w + seq : 2 * (int64_t)w + (late ? 1 : 0);
 }
 
-// The slot of a sequence that one wave covers, where it leaves a partial too
-// (DecodeParams::partial = 2).
-__device__ inline int64_t whole_slot(const DecodeParams& p, int J, int w, int64_t seq) {
-  return (int64_t)p.B * J <= p.n_waves ? w + seq : 2 * (int64_t)p.n_waves + seq;
-}
-
 // Position in the stage list: batch b, sequence j = kv_head * n_hc + slice
 // within the batch, stage st of nst = ceil(L / SK).
 struct Cursor {
@@ -839,8 +833,7 @@ __global__ __launch_bounds__(64 * NWV) void pf_decode_stream_kernel(DecodeParams
       }
       const int kvh = n_hc == 1 ? cc.j : cc.j / n_hc, hc = cc.j - kvh * n_hc;
       const int qh = hc * 16 + i16;
-      const bool whole = piece_st0 == 0 && cc.st == cc.nst - 1;
-      if (whole && p.partial == 0) {
+      if (piece_st0 == 0 && cc.st == cc.nst - 1) {
         // The whole sequence: finish it here.
         if (qh < g) {
           const float inv = (l_tot == 0.f) ? 0.f : 1.f / l_tot;
@@ -857,8 +850,7 @@ __global__ __launch_bounds__(64 * NWV) void pf_decode_stream_kernel(DecodeParams
           }
         }
       } else if (i16 < QR) {
-        const int64_t seq = (int64_t)cc.b * J + cc.j;
-        const int64_t pslot = whole ? whole_slot(p, J, w, seq) : piece_slot(p, J, w, seq, !first_piece);
+        const int64_t pslot = piece_slot(p, J, w, (int64_t)cc.b * J + cc.j, !first_piece);
         float* po = p.part_o + (pslot * QR + i16) * D;
 #pragma unroll
         for (int q = 0; q < G::NACC; ++q) {
@@ -903,12 +895,6 @@ __global__ __launch_bounds__(64 * NWV) void pf_decode_stream_kernel(DecodeParams
           o += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(smem_all + v * NS * kSlotB) + row * D + d0) *
                wt;
         }
-      }
-      if (p.partial != 0) {
-        const int64_t at = (int64_t)w * QR + row;
-        *reinterpret_cast<f32x4*>(p.part_o + at * D + d0) = o;
-        if (d0 == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * at) = (f32x2){M, l};
-        continue;
       }
       const float inv = (l == 0.f) ? 0.f : 1.f / l;
       typedef T v4 __attribute__((ext_vector_type(4)));
@@ -1178,20 +1164,19 @@ hipError_t launch_combine(const DecodeParams& p, hipStream_t st) {
 // 5.1-6.6 us; from about 16 stages the longer chain costs what the second
 // kernel did. A grid size set by hand (decode_waves) keeps the persistent grid.
 constexpr int kShortWaves = 4, kShortStages = 12;
-template <typename T, int D, int QR>
-bool short_form(const DecodeParams& p, bool paged) {
+template <typename T, int D, int PG, int QR>
+bool short_form(const DecodeParams& p) {
   using G = StreamGeo<T, D>;
   const int64_t seqs = (int64_t)p.B * p.Hkv * ((p.Hq / p.Hkv + 15) / 16);
-  const int64_t len = !paged ? p.cache_len : (int64_t)p.pages_per_seq * p.page_size;
+  const int64_t len = PG <= 1 ? p.cache_len : (int64_t)p.pages_per_seq * p.page_size;
   constexpr int per_cu = 160 * 1024 / (kShortWaves * 2 * G::slot_bytes(QR));
-  return per_cu > 0 && !p.fine && !p.fixed_grid && p.stages == 2 && seqs <= 256 * per_cu &&
-         len <= kShortStages * G::SK;
+  return per_cu > 0 && !p.fixed_grid && p.stages == 2 && seqs <= 256 * per_cu && len <= kShortStages * G::SK;
 }
 
 template <typename T, int D, int PG, int NS, int QR, bool FINE>
 hipError_t launch_stream(const DecodeParams& p, hipStream_t st) {
   if constexpr (!FINE && NS == 2 && kShortWaves * 2 * StreamGeo<T, D>::slot_bytes(QR) <= 160 * 1024) {
-    if (short_form<T, D, QR>(p, PG > 1)) {
+    if (short_form<T, D, PG, QR>(p)) {
       const unsigned seqs = (unsigned)(p.B * p.Hkv * ((p.Hq / p.Hkv + 15) / 16));
       hipLaunchKernelGGL((pf_decode_stream_kernel<T, D, PG, 2, QR, kShortWaves>), dim3(seqs), dim3(64 * kShortWaves),
                          0, st, p);
@@ -1201,7 +1186,7 @@ hipError_t launch_stream(const DecodeParams& p, hipStream_t st) {
   hipLaunchKernelGGL((pf_decode_stream_kernel<T, D, PG, NS, QR, 1, FINE>), dim3((unsigned)p.n_waves), dim3(64), 0, st,
                      p);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.partial != 0) return e;
+  if (e != hipSuccess) return e;
   return launch_combine<T, D, PG, QR, FINE>(p, st);
 }
 

@@ -290,12 +290,6 @@ struct DecodeParams {
   int slice;          // generic kernel: batches per launch
   int full_waves;     // streaming kernel: the waves that are resident at once (host only)
   int n_waves;        // streaming kernel: persistent grid (one wave per workgroup); 0: generic kernel
-  // Sequences of a shared-prefix call (attn_prefix.hip): every sequence leaves its
-  // partials, whole ones too, and no second kernel runs. Streaming kernel: 1, a
-  // workgroup per sequence and slot `sequence`; 2, the persistent grid and slots
-  // piece_slot / whole_slot. Generic kernel: 1 as 2. 0: a call of its own.
-  int partial;
-  int qrows;          // query rows per partial slot, for the merge
   // Fused decode step (streaming kernel, positions != null): the new token of
   // batch b is at pos = positions[b * pos_stride]; its k (rotated with table
   // row pos) and v go to cache slot pos (ring: pos % cache_size) and it
@@ -326,9 +320,6 @@ int decode_stream_waves(int dtype, int head_dim, int stages, int group, bool fin
 int decode_stream_qrows(int group);               // query rows per partial slot
 hipError_t launch_decode_stream(const DecodeParams& p, int dtype, bool paged, hipStream_t stream);
 
-// Whether the streaming kernel runs this call a workgroup per sequence.
-bool decode_stream_short(const DecodeParams& p, int dtype, bool paged);
-
 // Attention of a batch over a shared prefix (attn_prefix.hip).
 constexpr int kPrefixRows = 128;     // query rows per workgroup
 constexpr int kPrefixGroups = 1024;  // page lookups a workgroup can hold
@@ -336,24 +327,30 @@ struct PrefixParams {
   const void* q;  // [B, Hq, dr]
   const void* k;  // page pools
   const void* v;
-  const int32_t* table;    // the prefix's pages
-  const int32_t* len_ptr;  // its length in device memory (at most len), or null: len
-  int len;
+  void* o;
   int B, Hq, Hkv, g, rows;  // rows = B g
   int dr;                   // stored head dim
   int num_pages, page_size;
   int dma;         // whole loads lie inside a page and the pools are aligned
   int group_log2;  // keys of one page lookup (a power of two that divides page_size, at most 64)
-  int n_tiles;     // ceil(rows / kPrefixRows)
-  int chunk;       // keys per chunk (a multiple of 64)
-  int n_split;     // ceil(len / chunk)
   float scale_log2;
-  float* part_o;   // [n_split, B, Hq, D]
-  float* part_ml;  // [n_split, B, Hq, 2]
+  // the prefix: chunks [0, n_split) of `chunk` keys (a multiple of 64)
+  const int32_t* table;
+  const int32_t* len_ptr;  // its length in device memory (at most len), or null: len
+  int len;
+  int n_tiles;             // ceil(rows / kPrefixRows)
+  int chunk, n_split;
+  int n_pre;               // work items: n_tiles Hkv n_split
+  // the sequences' own keys: chunks [n_split, n_split + n_own)
+  const int32_t* own_tables;  // [B, pages_per_seq]
+  const int32_t* own_lens;    // [B]
+  int pages_per_seq, own_cap;  // own_cap = pages_per_seq page_size
+  int own_chunk, n_own;
+  int n_hc;                // ceil(g / kPrefixRows)
+  float* part_o;   // [n_split + n_own, B, Hq, D]
+  float* part_ml;  // [n_split + n_own, B, Hq, 2]
 };
 hipError_t launch_prefix(const PrefixParams& p, int dtype, int D, hipStream_t stream);
-// own: the sequences' own part as it was launched (pages_per_seq 0: none)
-hipError_t launch_prefix_merge(const DecodeParams& own, const PrefixParams& p, int dtype, int D, hipStream_t stream);
 
 // Cache writes (cache_ops.hip). positions: device int32, read at
 // b * pos_stride (pos_stride 0 = one position for the whole batch).
