@@ -113,6 +113,12 @@ CASES = [  # batch, hq, hkv, d, page, prefix, lens
     (3, 6, 2, 128, 50, 1111, [49, 50, 51]),
     (2, 14, 2, 64, 12, 1000, [1000, 12]),
     (6, 16, 4, 64, 16, 2000, [0, 300, 1, 16, 15, 17]),
+    (3, 8, 1, 128, 12, 90, [1, 40, 200]),
+    (3, 16, 2, 64, 8, 90, [1, 40, 200]),
+    (2, 14, 2, 64, 12, 90, [33, 40]),
+    (2, 9, 1, 128, 16, 90, [33, 400]),
+    (2, 260, 2, 64, 16, 90, [33, 400]),
+    (70, 5, 5, 128, 20, 33, [i % 7 for i in range(70)]),
 ]
 
 
@@ -129,6 +135,8 @@ def test_against_float64(batch, hq, hkv, d, page, prefix, lens, dt):
     (17, 16, 1, 256, 2, 260, [9 * i for i in range(17)]),
     (2, 4, 2, 200, 32, 333, [70, 129]),
     (2, 4, 2, 136, 7, 100, [70, 13]),
+    (5, 8, 1, 256, 4, 100, [70, 13, 0, 1, 300]),
+    (5, 8, 1, 256, 6, 100, [70, 13, 0, 1, 300]),
 ])
 def test_wide_heads(batch, hq, hkv, d, page, prefix, lens, dt):
     note(f"prefix {dt} B={batch} {hq}/{hkv} D={d} page={page} prefix={prefix}")

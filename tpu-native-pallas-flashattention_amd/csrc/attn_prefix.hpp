@@ -1,0 +1,869 @@
+// Single-query attention of a batch that shares a prefix (gfx950): every
+// sequence attends the prefix's pages and then its own.
+//
+//   o_b = softmax(scale q_b [K_prefix; K_b]^T) [V_prefix; V_b]
+//
+// A paged decode reads the prefix once per sequence. Here the B g query rows
+// of a KV head (all sequences, g heads each) are one matrix against it. Two
+// launches:
+//  * pf_prefix_kernel. Its first workgroups take a prefix item each: 128 rows
+//    of a KV head against one chunk of the prefix's keys. The others share the
+//    sequences' own keys: the streaming decode's work list (decode_stream.hpp),
+//    a contiguous run of it each, whatever the lengths. Prefix items are bound
+//    by the matrix cores where there are many sequences, own keys by memory;
+//    both kinds run beside each other. Each leaves (max, sum, acc) of its rows
+//    in float32 for every chunk or piece.
+//  * pf_prefix_merge_kernel: o = sum_i acc_i 2^(m_i - M) / sum_i l_i 2^(m_i - M)
+//    over a row's chunks and pieces.
+// No counterpart in the reference, whose paged call gives the prefix's pages
+// to every sequence's table (paged.py:102-192).
+//
+// A prefix item runs the prefill forward's pipeline (attn_fwd.hip) over pages: K
+// one 64-key block ahead of V, both double-buffered in LDS; S^T = K Q^T runs
+// beside the exponentials of the block before, O^T += V^T P^T beside the maximum
+// of the block after. The tiles come by direct global -> LDS loads of whole rows
+// (1 KB each, inside one page; rows past the length and columns past the stored
+// head dim lie outside the load's buffer range and arrive as zeros); a block's
+// pages are looked up one block before its loads. Pages that such loads would
+// straddle and unaligned pools are staged through registers instead.
+//
+// Own keys with at most 8 heads a KV head: the workgroup's waves each stream a
+// run of their own (own_stream). More heads, stored head dims that are not a
+// kernel's, odd pages and unaligned operands: the workgroup runs the prefix
+// items' pipeline over its run, across the sequences: the block after a
+// sequence's last one is the next sequence's first.
+#pragma once
+
+#include "decode_stream.hpp"
+#include "pf_common.hpp"
+#include "pf_kernels.hpp"
+#include "pf_tiles.hpp"
+
+namespace pf {
+
+namespace prefix {
+
+constexpr int kBN = 64;      // keys per block
+constexpr int kRows = kPrefixRows;
+
+constexpr int kPG = 2;  // the work list's lengths are those of a paged call
+using stream::Cursor;
+
+__device__ inline int prefix_len(const PrefixParams& p) {
+  return p.len_ptr != nullptr ? min(max(stream::sload_i32(p.len_ptr, 0), 0), p.len) : p.len;
+}
+
+// Slot of an own piece of sequence seq that workgroup w leaves; whole: all of the
+// sequence. Few sequences: w + seq names every piece once (stream::piece_slot).
+// Many: a workgroup leaves at most a piece that opens its run and one that closes
+// it, and whole sequences have slots of their own.
+__device__ inline int64_t own_slot(const DecodeParams& p, int J, int w, int64_t seq, bool whole, bool late) {
+  if (whole && (int64_t)p.B * J > p.n_waves) return 2 * (int64_t)p.n_waves + seq;
+  return stream::piece_slot(p, J, w, seq, late);
+}
+
+// Loads of 64-row tiles: the keys [64 st, ...) below L of the cursor's sequence.
+// DMA: each wave's loads are RPL whole rows of one page; else every lane fetches
+// its 16-byte chunks itself.
+template <typename T, int D, bool DMA>
+struct PageTiles {
+  using G = Tile<T, D>;
+  static constexpr int PT = G::CPR / 4;         // loads per lane and tile
+  static constexpr int RPL = 1024 / G::RB;      // rows per load
+  uint32_t voff[PT];  // DMA: the lane's byte offset within the load's rows
+  uint32_t row0;      // DMA: the wave's first row of load 0; load u: + 4 RPL u
+  uint32_t slot0;     // the wave's LDS byte offset of load 0; load u: + 4096 u
+  int lane, n_hc;
+  const PrefixParams& p;
+  const int32_t* table;  // of the prefix, or all sequences'
+  int pages;             // per sequence
+
+  __device__ inline PageTiles(const PrefixParams& p_, int tid, bool own)
+      : lane(tid & 63), n_hc(own ? p_.n_hc : 1), p(p_), table(own ? p_.own.block_tables : p_.table),
+        pages(own ? p_.own.pages_per_seq : p_.pages) {
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    row0 = RPL * w;
+    slot0 = 1024 * w;
+#pragma unroll
+    for (int u = 0; u < PT; ++u) {
+      const int r = lane / G::CPR, row = RPL * (4 * u + w) + r;
+      const int chunk = (lane % G::CPR) ^ tile_swz<G::CPR>(row);
+      // columns past the stored row: past any range
+      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((r * p.dr + chunk * G::EPC) * G::ES) : 0x7ffffff0u;
+    }
+  }
+  __device__ inline int kv_head(const Cursor& c) const { return n_hc == 1 ? c.j : c.j / n_hc; }
+  // The page lookups of the wave's loads of a block, load u in lane u: the
+  // entry, and where the load starts in the page. A load past the table's reach
+  // looks up the last page and reads nothing.
+  struct Look {
+    int page;
+    uint32_t off;
+  };
+  __device__ inline Look look(const Cursor& c) const {
+    const int key = kBN * c.st + row0 + 4 * RPL * (lane & (PT - 1));
+    const int lp = min((int)fast_div(key, p.div_page), pages - 1);
+    return Look{table[(int64_t)c.b * pages + lp], (uint32_t)(key - lp * p.page_size)};
+  }
+  // The pool rows where the loads start (in lane u), once the entries are there.
+  __device__ inline uint32_t rows(const Cursor& c, const Look& l) const {
+    const int page = min(max(l.page, 0), p.num_pages - 1);
+    return ((uint32_t)page * p.Hkv + kv_head(c)) * p.page_size + l.off;
+  }
+  __device__ inline void load(const void* pool, const Cursor& c, uint32_t rows, int u, char* tile) const {
+    const int key = kBN * c.st + row0 + 4 * RPL * u;
+    const int valid = min(max(c.L - key, 0), RPL);
+    const uint32_t rb = p.dr * G::ES;
+    const uint32_t row = __builtin_amdgcn_readlane(rows, u);
+    const i32x4 d = make_desc(static_cast<const char*>(pool) + (uint64_t)row * rb, valid * rb);
+    dma16<true>(d, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 4096 * u));
+  }
+  // Without DMA: a block through registers.
+  __device__ inline void copy(const void* pool, const Cursor& c, char* tile) const {
+    u32x4 x[PT];
+#pragma unroll
+    for (int u = 0; u < PT; ++u) {
+      const int s = (slot0 + 4096 * u) / 16 + lane, row = s / G::CPR;
+      const int chunk = (s % G::CPR) ^ tile_swz<G::CPR>(row), key = kBN * c.st + row;
+      x[u] = (u32x4){0u, 0u, 0u, 0u};
+      if (key < c.L && chunk * G::EPC < p.dr) {
+        const int lp = fast_div(key, p.div_page);
+        const int page = min(max(table[(int64_t)c.b * pages + lp], 0), p.num_pages - 1);
+        const int64_t at = ((int64_t)page * p.Hkv + kv_head(c)) * p.page_size + (key - lp * p.page_size);
+        x[u] = ldg16(static_cast<const T*>(pool) + at * p.dr + chunk * G::EPC);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < PT; ++u) sts16(tile + slot0 + 4096 * u + 16 * lane, x[u]);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Own keys, at most 8 query heads per KV head: wave w of own.n_waves streams its
+// run of the work list in stages of 16 keys through a ring of two stages in LDS,
+// with no barrier: 16x16 MFMAs, S^T (16 keys x heads) and O^T += V^T P^T, as the
+// streaming decode. A stage's K is free once its scores are there, its V once
+// P.V is, and each is refilled right then with the stage two on: two stages are
+// in flight nearly always, 64 KB of a workgroup's four waves at head_dim 128.
+// (Half of that, refilled stage by stage, or the prefix pipeline over 64-key
+// blocks, is what leaves a CU that also computes a prefix item short of memory
+// traffic.) A sequence's query rows come the same way, with its first stage.
+// PG: rows of one page lookup (page_size % PG == 0).
+// ---------------------------------------------------------------------------
+constexpr int kOwnKeys = 16;   // keys per stage
+constexpr int kOwnHeads = 8;   // query rows per sequence, at most
+
+template <typename T, int D>
+struct OwnGeo {
+  static constexpr int RB = D * (int)sizeof(T);  // row bytes: 128, 256 or 512
+  static constexpr int CPR = RB / 16;            // chunks per row
+  static constexpr int TILE = kOwnKeys * RB;     // a stage of K (or V)
+  static constexpr int NL = TILE / 1024;         // loads per tile
+  static constexpr int RPL = 1024 / RB;          // rows per load
+  static constexpr int QB = kOwnHeads * RB;      // query rows
+  static constexpr int WAVE = 4 * TILE + 2 * QB;  // K, V: two stages each; Q: two sequences
+  static_assert(RB == 128 || RB == 256 || RB == 512, "row sizes");
+  // Chunk permutation of row r (XOR of the low bits of the chunk index): the 16
+  // rows of a K read hit 16 bank groups (128-byte rows: row bit 0 already parts
+  // two rows of a bank window), and so do the 4 rows x 2 chunks of a V read.
+  __host__ __device__ static constexpr int swz(int r) {
+    if (RB == 128) return (((r >> 1) & 1) << 1) | ((r >> 3) & 1) | (((r >> 2) & 1) << 2);
+    return ((r >> 2) & 1) | ((r & 3) << 1) | (((r >> 3) & 1) << 3);
+  }
+  static constexpr int QMASK = (CPR < 16 ? CPR : 16) - 1;  // query row permutation
+};
+
+// The wave's LDS reads so far have their data (what they read may be overwritten).
+__device__ inline void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+template <typename T, int D, int PG>
+__device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, int w) {
+  using MF = stream::Mfma16<T>;
+  using G = OwnGeo<T, D>;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int SK = kOwnKeys, RB = G::RB, NL = G::NL, NSTEP = G::CPR / 4, NACC = D / 16;
+  constexpr int kGroups = SK / PG, kPer = NL / kGroups;
+  static_assert(PG % G::RPL == 0 && SK % PG == 0, "a page group is whole loads of one stage");
+  const DecodeParams& own = p.own;
+  const int lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
+  const int g = p.g, J = p.Hkv, ps = p.page_size;
+
+  if (w >= own.n_waves) return;
+  Cursor cc;
+  stream::Partition part((int64_t)0, (int64_t)0);
+  const int64_t n = stream::wave_plan<kPG, SK>(own, J, own.n_waves, w, &cc, &part);
+  if (n <= 0) return;
+
+  char* const kbuf = ring;                 // stages k & 1
+  char* const vbuf = ring + 2 * G::TILE;
+  char* const qbuf = ring + 4 * G::TILE;   // sequences in turn
+
+  // The chunk that this lane fetches for load i: its byte offset within the page group.
+  uint32_t loff[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int row = G::RPL * i + lane / G::CPR, c = lane % G::CPR;
+    loff[i] = (uint32_t)((row % PG) * RB + 16 * (c ^ G::swz(row)));
+  }
+  // A stage's page groups: pool row and valid rows of each. Groups past the
+  // length load nothing and look nothing up (-1 padding).
+  struct Stage {
+    uint32_t row[kGroups];
+    int valid[kGroups];
+  };
+  auto look = [&](const Cursor& c) {
+    Stage s;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int key = c.st * SK + i * PG;
+      s.valid[i] = min(max(c.L - key, 0), PG);
+      const int lp = s.valid[i] > 0 ? (int)fast_div(key, p.div_page) : 0;
+      int page = s.valid[i] > 0 ? stream::sload_i32(own.block_tables, (int64_t)c.b * own.pages_per_seq + lp) : 0;
+      page = min(max(page, 0), p.num_pages - 1);
+      s.row[i] = ((uint32_t)page * p.Hkv + c.j) * ps + (s.valid[i] > 0 ? key - lp * ps : 0);
+    }
+    return s;
+  };
+  auto load = [&](const void* pool, const Stage& s, char* tile) {
+    const uint32_t at = lds_u32(tile);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const i32x4 d = make_desc(static_cast<const char*>(pool) + (uint64_t)s.row[i] * RB, s.valid[i] * RB);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) dma16<true>(d, loff[i * kPer + e], at + 1024 * (i * kPer + e));
+    }
+  };
+  auto load_q = [&](const Cursor& c, char* q) {
+    const i32x4 d = make_desc(static_cast<const T*>(p.q) + ((int64_t)c.b * p.Hq + (int64_t)c.j * g) * D, g * RB);
+#pragma unroll
+    for (int i = 0; i < G::QB / 1024; ++i) {
+      const int row = G::RPL * i + lane / G::CPR, c16 = lane % G::CPR;
+      dma16(d, (uint32_t)(row * RB + 16 * (c16 ^ (row & G::QMASK))), lds_u32(q) + 1024 * i);
+    }
+  };
+
+  // Prologue: stages 0 and 1. pc: the stage that is loaded next.
+  Cursor pc = cc;
+  int q_in = 0, q_out = 0;  // sequences whose queries were asked for, and taken
+  load_q(cc, qbuf);
+  ++q_in;
+  Stage st = look(cc);
+  load(p.k, st, kbuf);
+  load(p.v, st, vbuf);
+  stream::cursor_next<kPG, SK>(pc, own, J);
+  if (n > 1) {
+    st = look(pc);
+    if (pc.st == 0) load_q(pc, qbuf + G::QB * (q_in++ & 1));
+    load(p.k, st, kbuf + G::TILE);
+    load(p.v, st, vbuf + G::TILE);
+    stream::cursor_next<kPG, SK>(pc, own, J);
+  }
+
+  // LDS read offsets. K (A operand of S^T): row i16, chunk 4s + h; past 16 chunks
+  // 256 bytes on. V: 16-bit, transposing reads of rows 4h + i16/4, columns 16dt +
+  // 4(i16%4) .. + 3; float32, row 4h + e, chunk i16.
+  constexpr int NKO = NSTEP < 4 ? NSTEP : 4, NVO = F32 ? 4 : (NACC < 8 ? NACC : 8);
+  uint32_t koff[NKO], voff[NVO];
+#pragma unroll
+  for (int s = 0; s < NKO; ++s) koff[s] = (uint32_t)(i16 * RB + 16 * ((4 * s + h) ^ G::swz(i16)));
+#pragma unroll
+  for (int e = 0; e < NVO; ++e) {
+    if constexpr (F32) {
+      voff[e] = (uint32_t)((4 * h + e) * RB + 16 * (i16 ^ G::swz(4 * h + e)));
+    } else {
+      const int row = 4 * h + (i16 >> 2), chunk = 2 * e + ((i16 >> 1) & 1);
+      voff[e] = (uint32_t)(row * RB + 16 * (chunk ^ G::swz(row)) + 8 * (i16 & 1));
+    }
+  }
+
+  u32x4 qf[NSTEP];
+  // O^T: 16-bit tile dt, register r = column 16dt + 4h + r; float32 tile 4 blk + e,
+  // register r = column 64 blk + 16h + 4r + e. Column i16: head i16.
+  f32x4 acc[NACC];
+  float m_run = -__FLT_MAX__, l_run = 0.f;  // as the prefix items
+  int piece_st0 = 0;
+  bool first_piece = true;
+
+  for (int64_t k = 0; k < n; ++k) {
+    // Loads complete in order: all but the next stage's (queries with its first
+    // one included) are there.
+    if (k + 1 < n) wait_vm<2 * NL>();
+    else wait_vm<0>();
+    char* const sK = kbuf + (k & 1) * G::TILE;
+    char* const sV = vbuf + (k & 1) * G::TILE;
+    if (k == 0 || cc.st == 0) {
+      const char* sQ = qbuf + G::QB * (q_out++ & 1);
+#pragma unroll
+      for (int s = 0; s < NSTEP; ++s)
+        qf[s] = i16 < kOwnHeads ? lds16(sQ + i16 * RB + 16 * ((4 * s + h) ^ (i16 & G::QMASK)))
+                                : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int a = 0; a < NACC; ++a) acc[a] = (f32x4)(0.f);
+      m_run = -__FLT_MAX__;
+      l_run = 0.f;
+      piece_st0 = cc.st;
+    }
+    f32x4 s = (f32x4)(0.f);  // keys 4h + r, head i16
+#pragma unroll
+    for (int e = 0; e < NSTEP; ++e) s = MF::run(lds16(sK + koff[e % NKO] + 256 * (e / NKO)), qf[e], s);
+
+    const bool more = k + 2 < n;
+    if (more) {
+      st = look(pc);
+      wait_lds();  // K and Q are read
+      if (pc.st == 0) load_q(pc, qbuf + G::QB * (q_in++ & 1));
+      load(p.k, st, sK);
+    }
+
+    float x[4], mx = kNegInf;
+    const int rel = cc.L - cc.st * SK - 4 * h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x[t] = t < rel ? s[t] * p.scale_log2 : kNegInf;
+      mx = fmaxf(mx, x[t]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = wave_xor32_max(mx);
+    const float m_cand = fmaxf(m_run, mx);
+    if (__any(m_cand > m_run + 8.f)) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_cand);
+#pragma unroll
+      for (int a = 0; a < NACC; ++a) acc[a] *= alpha;
+      l_run *= alpha;
+      m_run = m_cand;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x[t] = __builtin_amdgcn_exp2f(x[t] - m_run);
+      l_run += x[t];
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int blk = 0; blk < D / 64; ++blk) {
+          const f32x4 v = __builtin_bit_cast(f32x4, lds16(sV + voff[t] + 256 * blk));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[4 * blk + e] = MF::step(v[e], x[t], acc[4 * blk + e]);
+        }
+    } else {
+      const u32x2 pf = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};  // half a step of each weight
+#pragma unroll
+      for (int dt = 0; dt < NACC; ++dt) {
+        const stream::i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) stream::i16x4*)(sV + voff[dt % NVO] + 256 * (dt / NVO)));
+        acc[dt] = MF::run16(__builtin_bit_cast(u32x2, v), pf, acc[dt]);
+      }
+    }
+    if (more) {
+      wait_lds();  // V is read
+      load(p.v, st, sV);
+      stream::cursor_next<kPG, SK>(pc, own, J);
+    }
+
+    if (cc.st == cc.nst - 1 || k == n - 1) {
+      float l_tot = l_run + __shfl_xor(l_run, 16);
+      l_tot = wave_xor32_sum(l_tot);
+      if (i16 < g) {
+        const bool whole = piece_st0 == 0 && cc.st == cc.nst - 1;
+        const int64_t at = own_slot(own, J, w, (int64_t)cc.b * J + cc.j, whole, !first_piece) * g + i16;
+        float* po = own.part_o + at * D;
+#pragma unroll
+        for (int q = 0; q < NACC; ++q) {
+          if constexpr (F32) {
+            const int blk = q >> 2, r = q & 3;
+            *reinterpret_cast<f32x4*>(po + 64 * blk + 16 * h + 4 * r) =
+                (f32x4){acc[4 * blk][r], acc[4 * blk + 1][r], acc[4 * blk + 2][r], acc[4 * blk + 3][r]};
+          } else {
+            *reinterpret_cast<f32x4*>(po + 16 * q + 4 * h) = acc[q];
+          }
+        }
+        if (h == 0) *reinterpret_cast<f32x2*>(own.part_ml + 2 * at) = (f32x2){m_run, l_tot};
+      }
+      first_piece = false;
+    }
+    stream::cursor_next<kPG, SK>(cc, own, J);
+  }
+}
+
+// PG > 0: own keys by own_stream; 0: by the block pipeline.
+template <typename T, int D, bool DMA, int PG>
+__global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(PrefixParams p) {
+  using MF = Mfma32<T>;
+  using Frag = typename MF::Frag;
+  using G = Tile<T, D>;
+  using PTiles = PageTiles<T, D, DMA>;
+  constexpr int HALF = D / 2, EPC = G::EPC, FPC = frags_per_chunk<T>();
+  constexpr int QF = HALF / MF::kK, NDT = D / 32, PF = 32 / MF::kK, PT = PTiles::PT;
+  // K blocks t & 1, then V blocks; or the waves' rings
+  static_assert(4 * OwnGeo<T, D>::WAVE >= 4 * G::BYTES, "the rings hold two blocks");
+  __shared__ __attribute__((aligned(1024))) char smem[PG > 0 ? 4 * OwnGeo<T, D>::WAVE : 4 * G::BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hh = lane >> 5, l32 = lane & 31;
+  const bool own_wg = blockIdx.x >= (unsigned)p.n_pre;
+  if constexpr (PG > 0) {
+    if (own_wg) {
+      own_stream<T, D, PG>(p, smem + wv * OwnGeo<T, D>::WAVE, 4 * (blockIdx.x - p.n_pre) + wv);
+      return;
+    }
+  }
+  const bool own = PG == 0 && own_wg;
+  const int J = p.Hkv * p.n_hc;
+
+  // The workgroup's n blocks and the first one's cursor.
+  Cursor cp;
+  int n, r0 = 0, piece = 0;
+  if (!own) {
+    // (chunk, kv head, row tile): the row tiles of one chunk side by side on one
+    // XCD, whose L2 then serves the chunk to all of them.
+    const int item = xcd_remap(blockIdx.x, p.n_pre, p.n_tiles);
+    r0 = kRows * (item % p.n_tiles);
+    piece = item / p.n_tiles / p.Hkv;
+    const int key0 = piece * p.chunk, L = min(prefix_len(p), key0 + p.chunk);
+    n = (L - key0 + kBN - 1) / kBN;
+    cp = Cursor{0, item / p.n_tiles % p.Hkv, key0 / kBN, key0 / kBN + n, L};
+  } else {
+    stream::Partition part((int64_t)0, (int64_t)0);
+    n = (int)stream::wave_plan<kPG, kBN>(p.own, J, p.own.n_waves, blockIdx.x - p.n_pre, &cp, &part);
+  }
+  if (n <= 0) return;
+
+  const PTiles tiles(p, tid, own);
+  char* const kbuf0 = smem;
+  char* const vbuf0 = smem + 2 * G::BYTES;
+  auto next = [&](Cursor& c) { stream::cursor_next<kPG, kBN>(c, p.own, J); };
+
+  // An own block seldom has rows for more than one wave: which one differs from
+  // workgroup to workgroup, so that those on a CU load all of its SIMDs.
+  const int w32 = 32 * (own ? (wv + blockIdx.x) & 3 : wv);
+  // The lane's query row in the cursor's sequence: (batch, head) index, or -1.
+  auto row_of = [&](const Cursor& c) -> int {
+    if (!own) {
+      const int r = r0 + w32 + l32;
+      if (r >= p.rows) return -1;
+      const int b = r / p.g;
+      return b * p.Hq + c.j * p.g + (r - b * p.g);
+    }
+    const int kvh = tiles.kv_head(c), r = kRows * (c.j - kvh * p.n_hc) + w32 + l32;
+    return r < p.g ? c.b * p.Hq + kvh * p.g + r : -1;
+  };
+  // Whether the wave has rows at all: of an own sequence's slices only the last
+  // can be short, so a wave without rows there may have some in others.
+  const bool active = own ? w32 < p.own_rows : r0 + w32 < p.rows;
+
+  u32x4 qc[HALF / EPC];  // Q: the lane's row, columns [hh HALF, + HALF)
+  auto load_q = [&](const Cursor& c) {
+    const int r = row_of(c);
+    const T* qr = static_cast<const T*>(p.q) + (int64_t)r * p.dr + hh * HALF;
+#pragma unroll
+    for (int i = 0; i < HALF / EPC; ++i)
+      qc[i] = r >= 0 && hh * HALF + i * EPC < p.dr ? ldg16(qr + i * EPC) : (u32x4){0u, 0u, 0u, 0u};
+  };
+  // A negative scale is applied as |scale| on -Q.
+  auto sign_q = [&]() {
+    if (p.scale_log2 < 0.f) {
+      const uint32_t sign = G::ES == 4 ? 0x80000000u : 0x80008000u;
+#pragma unroll
+      for (int i = 0; i < HALF / EPC; ++i) qc[i] ^= (u32x4){sign, sign, sign, sign};
+    }
+  };
+  auto frags = [&](Frag* qf) {
+#pragma unroll
+    for (int i = 0; i < HALF / EPC; ++i)
+#pragma unroll
+      for (int f = 0; f < FPC; ++f) qf[i * FPC + f] = chunk_frag<T>(qc[i], f);
+  };
+
+  // Cursors of blocks t (cp), t + 1 (cs), t + 2 (ck); rv, lk: the pool rows of
+  // block t + 1 and the lookups of block t + 2.
+  Cursor cs = cp, ck = cp;
+  if (n > 1) next(cs);
+  if (n > 2) {
+    ck = cs;
+    next(ck);
+  }
+  uint32_t rv = 0;
+  typename PTiles::Look lk{};
+  if constexpr (DMA) {
+    const typename PTiles::Look l0 = tiles.look(cp), l1 = tiles.look(cs);
+    lk = tiles.look(ck);
+    const uint32_t r0s = tiles.rows(cp, l0);
+    rv = tiles.rows(cs, l1);
+#pragma unroll
+    for (int u = 0; u < PT; ++u) tiles.load(p.k, cp, r0s, u, kbuf0);
+#pragma unroll
+    for (int u = 0; u < PT; ++u) tiles.load(p.v, cp, r0s, u, vbuf0);
+    if (n > 1) {
+#pragma unroll
+      for (int u = 0; u < PT; ++u) tiles.load(p.k, cs, rv, u, kbuf0 + G::BYTES);
+    }
+  } else {
+    tiles.copy(p.k, cp, kbuf0);
+    tiles.copy(p.v, cp, vbuf0);
+    if (n > 1) tiles.copy(p.k, cs, kbuf0 + G::BYTES);
+  }
+  load_q(cp);
+
+  // Running maximum (log2 units) from the lowest finite value: scores of -inf
+  // weigh nothing and a row of nothing else keeps sum 0.
+  float m_run = -__FLT_MAX__, l_run = 0.f;
+  f32x16 acc[NDT];
+#pragma unroll
+  for (int i = 0; i < NDT; ++i) acc[i] = (f32x16)(0.f);
+  const float c2 = fmaxf(fabsf(p.scale_log2), 1e-30f);  // masked scores (-inf) stay -inf
+  TrAddr<T, D> vta;
+  vta.init(lane);
+
+  // m_run moves when some row's maximum grows by more than 8: p <= 2^8, and the
+  // rescaling is rare.
+  auto update_max = [&](float mx) {
+    const float m_cand = fmaxf(m_run, mx);
+    if (__any(m_cand > m_run + 8.f)) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_cand);
+#pragma unroll
+      for (int i = 0; i < NDT; ++i) acc[i] *= alpha;
+      l_run *= alpha;
+      m_run = m_cand;
+    }
+  };
+  // The lane's maximum of a block's scores; keys at or past L become -inf.
+  auto block_max = [&](f32x16* s, const Cursor& c) {
+    const int rel = c.L - kBN * c.st - 32 * hh;
+    float mx = kNegInf;
+#pragma unroll
+    for (int v = 0; v < 32; ++v) {
+      const float x = v < rel ? s[v >> 4][v & 15] : kNegInf;
+      s[v >> 4][v & 15] = x;
+      mx = fmaxf(mx, x);
+    }
+    return mx;
+  };
+  // The end of a chunk or piece: its partials, and a fresh state.
+  bool first_piece = true;
+  int piece_st0 = cp.st;
+  auto finish = [&](const Cursor& c) {
+    const float l_tot = wave_xor32_sum(l_run);
+    const int r = row_of(c);
+    if (r >= 0) {
+      float *po = p.part_o, *pm = p.part_ml;
+      int64_t at = (int64_t)piece * p.own.B * p.Hq + r;
+      if (own) {
+        const int w = blockIdx.x - p.n_pre;
+        const int64_t seq = (int64_t)c.b * J + c.j;
+        const bool whole = piece_st0 == 0 && c.st == c.nst - 1;
+        at = own_slot(p.own, J, w, seq, whole, !first_piece) * p.own_rows + w32 + l32;
+        po = p.own.part_o;
+        pm = p.own.part_ml;
+      }
+      store_acc_row<float, D>(po + at * D, acc, 1.f, hh);
+      if (hh == 0) *reinterpret_cast<f32x2*>(pm + 2 * at) = (f32x2){m_run, l_tot};
+    }
+    first_piece = false;
+    piece_st0 = 0;
+    m_run = -__FLT_MAX__;
+    l_run = 0.f;
+#pragma unroll
+    for (int i = 0; i < NDT; ++i) acc[i] = (f32x16)(0.f);
+  };
+
+  dma_wait();
+  __syncthreads();
+  f32x16 s_cur[2] = {(f32x16)(0.f), (f32x16)(0.f)};
+  float mx_carry = kNegInf;  // the lane's maximum of the latest block, not yet applied
+  if (active) {
+    sign_q();
+    Frag qf[QF];
+    frags(qf);
+    mfma_nat<T, D>(kbuf0, l32, hh, qf, s_cur[0], s_cur[1]);
+    mx_carry = block_max(s_cur, cp);
+    if (own && n > 1 && cs.st == 0) {
+      load_q(cs);
+      sign_q();
+    }
+  }
+  __syncthreads();  // K_0 is read before K_2 overwrites it
+
+  for (int t = 0; t + 1 < n; ++t) {
+    char* const kcur = kbuf0 + ((t + 1) & 1) * G::BYTES;  // K_{t+1}
+    char* const vcur = vbuf0 + (t & 1) * G::BYTES;        // V_t
+    char* const kdst = kbuf0 + (t & 1) * G::BYTES;        // K_{t+2}
+    char* const vdst = vbuf0 + ((t + 1) & 1) * G::BYTES;  // V_{t+1}
+    const bool k_next = t + 2 < n;
+    Cursor cl = ck;  // block t + 3
+    if (t + 3 < n) next(cl);
+    uint32_t rk = 0;
+    auto load_part = [&](int i) __attribute__((always_inline)) {
+      if constexpr (DMA) {
+        if (i < PT) {
+          if (k_next) tiles.load(p.k, ck, rk, i, kdst);
+        } else if (i < 2 * PT) {
+          tiles.load(p.v, cs, rv, i - PT, vdst);
+        }
+      }
+    };
+    if constexpr (DMA) {
+      rk = tiles.rows(ck, lk);
+      lk = tiles.look(cl);
+    } else {
+      if (k_next) tiles.copy(p.k, ck, kdst);
+      tiles.copy(p.v, cs, vdst);
+    }
+    const bool new_q = own && k_next && ck.st == 0;  // block t + 2 opens a sequence
+    if (!active) {
+#pragma unroll
+      for (int i = 0; i < 2 * PT; ++i) load_part(i);
+    } else {
+      f32x16 s_nxt[2] = {(f32x16)(0.f), (f32x16)(0.f)};
+      Frag qf[QF], pfr[PF];
+      frags(qf);
+      const bool masked = (cs.st + 1) * kBN > cs.L;
+      if constexpr (sizeof(T) == 2) {
+        // As in the forward: S_{t+1} beside the maximum and the first quarter of
+        // S_t's exponentials, P.V beside the rest.
+        constexpr int NV1 = G::CPR, NV2 = 4 * NDT, VPS2 = 32 / NV2;
+        uint32_t pw[16];
+        float rs = 0.f, mxr = kNegInf, mx = kNegInf;
+        auto exp_pair = [&](int pr) __attribute__((always_inline)) {
+          const int v = 2 * pr;
+          const float x0 = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
+          const float x1 = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][(v & 15) + 1], c2, -m_run));
+          pw[pr] = pack2<T>(x0, x1);  // the matrix cores take P in T: half a step of each weight
+          rs += x0 + x1;              // the sum is of the unrounded weights
+          asm volatile("" : "+v"(rs));  // keeps the sum beside its MFMA
+        };
+        mfma_nat_il<T, D>(kcur, l32, hh, qf, s_nxt[0], s_nxt[1], [&](int i) {
+          load_part(i);
+          if (i == 0) {
+            mxr = wave_xor32_max(mx_carry) * c2;
+          } else if (i == 1) {
+            update_max(mxr);
+          } else {
+#pragma unroll
+            for (int pr = ((i - 2) * 4) / (NV1 - 2); pr < ((i - 1) * 4) / (NV1 - 2); ++pr) exp_pair(pr);
+          }
+        });
+        if (new_q) load_q(ck);  // Q is free now; there by the end of the block
+        pfr[0] = __builtin_bit_cast(Frag, (u32x4){pw[0], pw[1], pw[2], pw[3]});
+        mfma_trn_il<T, D>(vcur, vta, pfr, acc, [&](int i) {
+#pragma unroll
+          for (int pr = 4; pr < 16; ++pr) {
+            const int f = pr >> 2, q4 = pr & 3;
+            if (i == (f - 1) * NDT + (q4 * NDT) / 4) {
+              exp_pair(pr);
+              if (q4 == 3)
+                pfr[f] = __builtin_bit_cast(Frag, (u32x4){pw[4 * f], pw[4 * f + 1], pw[4 * f + 2], pw[4 * f + 3]});
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < VPS2; ++e) {
+            const int v = i * VPS2 + e;
+            mx = fmaxf(mx, s_nxt[v >> 4][v & 15]);
+          }
+          asm volatile("" : "+v"(mx));
+        });
+        l_run += rs;
+        mx_carry = mx;
+        if (masked) mx_carry = block_max(s_nxt, cs);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * PT; ++i) load_part(i);
+        __builtin_amdgcn_sched_barrier(0);
+        update_max(wave_xor32_max(mx_carry) * c2);
+        mfma_nat<T, D>(kcur, l32, hh, qf, s_nxt[0], s_nxt[1]);
+        if (new_q) load_q(ck);
+        float rs = 0.f;
+#pragma unroll
+        for (int v = 0; v < 32; ++v) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
+          s_cur[v >> 4][v & 15] = x;
+          rs += x;
+        }
+        l_run += rs;
+        pack_frags<T>(s_cur[0], s_cur[1], pfr);
+        mfma_trn<T, D>(vcur, lane, vta, pfr, acc);
+        mx_carry = block_max(s_nxt, cs);
+      }
+      s_cur[0] = s_nxt[0];
+      s_cur[1] = s_nxt[1];
+      if (own && cp.st == cp.nst - 1) finish(cp);
+    }
+    dma_wait();
+    if (new_q && active) sign_q();
+    __syncthreads();
+    cp = cs;
+    cs = ck;
+    ck = cl;
+    rv = rk;
+  }
+  if (!active) return;
+
+  update_max(wave_xor32_max(mx_carry) * c2);
+  {
+    Frag pfr[PF];
+    float rs = 0.f;
+#pragma unroll
+    for (int v = 0; v < 32; ++v) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
+      s_cur[v >> 4][v & 15] = x;
+      rs += x;
+    }
+    l_run += rs;
+    pack_frags<T>(s_cur[0], s_cur[1], pfr);
+    mfma_trn<T, D>(vbuf0 + ((n - 1) & 1) * G::BYTES, lane, vta, pfr, acc);
+  }
+  finish(cp);
+}
+
+// The merge: a workgroup per (batch, kv head, 16 of its heads), D / 4 lanes a
+// row, 16 bytes each; where the rows leave lanes over, groups of lanes share the
+// chunks and pieces and join through LDS. One wave finds the sequence's pieces in
+// the work list. Bound by the partials' latency: 8 are in flight per lane.
+template <typename T, int D, int SK>
+__global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
+  constexpr int LPR = D / 4, NB = 8;
+  const int g = p.g, n16 = (g + 15) >> 4;
+  const int b = blockIdx.x / (p.Hkv * n16), j16 = blockIdx.x - b * p.Hkv * n16;
+  const int kvh = j16 / n16, h0 = 16 * (j16 - kvh * n16);  // heads [h0, + nq) of the group
+  const int nq = min(16, g - h0);
+  const int tid = threadIdx.x;
+  const int J = p.Hkv * p.n_hc, slice = h0 / kRows;
+  const int64_t seq = (int64_t)b * J + kvh * p.n_hc + slice;
+
+  __shared__ int found[3];  // own pieces, first workgroup, whether it starts inside that one's run
+  if (tid < 64) {
+    int np = 0, wa = 0;
+    bool late = false;
+    if (p.own.n_waves > 0) {
+      const stream::BatchScan sc = stream::batch_scan<kPG, SK>(p.own, J);
+      const int L = sc.per == 1 ? __builtin_amdgcn_readlane(sc.L, b) : stream::seq_len<kPG>(p.own, b);
+      const int nst = (L + SK - 1) / SK;
+      if (nst > 0) {
+        const stream::Partition part(sc.tot, p.own.n_waves);
+        const int64_t s0 = stream::stages_before<kPG, SK>(p.own, J, b, sc) + (seq - (int64_t)b * J) * nst;
+        wa = part.wave_of(s0);
+        np = part.wave_of(s0 + nst - 1) - wa + 1;
+        late = part.start(wa) < s0;
+      }
+    }
+    if (tid == 0) {
+      found[0] = np;
+      found[1] = wa;
+      found[2] = late;
+    }
+  }
+  __syncthreads();
+  const int np = found[0], wa = found[1];
+  const bool late = found[2] != 0;
+  const int npre = (prefix_len(p) + p.chunk - 1) / p.chunk;
+  const int total = npre + np;
+
+  __shared__ f32x4 so[256];
+  __shared__ f32x2 sm[256];
+  const int per = nq * LPR;
+  const int ngrp = per >= 256 ? 1 : 256 / per;
+  const int grp = per >= 256 ? 0 : tid / per;
+  for (int i0 = 0; i0 < per; i0 += 256) {  // one round where per <= 256
+    const int i = per >= 256 ? i0 + tid : tid - grp * per;
+    const bool on = i < per && grp < ngrp;
+    const int qi = on ? i / LPR : 0, d0 = on ? 4 * (i % LPR) : 0;
+    const int64_t bh = (int64_t)b * p.Hq + kvh * g + h0 + qi;
+    float M = kNegInf, l = 0.f;
+    f32x4 o = (f32x4)(0.f);
+    for (int c0 = grp; on && c0 < total; c0 += NB * ngrp) {
+      f32x2 ml[NB];
+      f32x4 v[NB];
+      float Mn = M;
+#pragma unroll
+      for (int c = 0; c < NB; ++c) {
+        const int s = c0 + c * ngrp;
+        ml[c] = (f32x2){kNegInf, 0.f};
+        v[c] = (f32x4)(0.f);
+        if (s < total) {
+          const float *po = p.part_o, *pm = p.part_ml;
+          int64_t row = (int64_t)s * p.own.B * p.Hq + bh;
+          if (s >= npre) {
+            const int i1 = s - npre;
+            po = p.own.part_o;
+            pm = p.own.part_ml;
+            row = own_slot(p.own, J, wa + i1, seq, np == 1, i1 == 0 && late) * p.own_rows + h0 - kRows * slice + qi;
+          }
+          ml[c] = *reinterpret_cast<const f32x2*>(pm + row * 2);
+          v[c] = *reinterpret_cast<const f32x4*>(po + row * D + d0);
+        }
+        Mn = fmaxf(Mn, ml[c][0]);
+      }
+      const float Mu = (Mn == kNegInf) ? 0.f : Mn;
+      const float back = exp2f(M - Mu);
+      o *= back;
+      l *= back;
+#pragma unroll
+      for (int c = 0; c < NB; ++c) {
+        const float wt = exp2f(ml[c][0] - Mu);
+        l += ml[c][1] * wt;
+        o += v[c] * wt;
+      }
+      M = Mn;
+    }
+    if (ngrp > 1) {
+      so[tid] = o;
+      sm[tid] = (f32x2){M, l};
+      __syncthreads();
+      if (grp != 0) return;
+      for (int k = 1; k < ngrp; ++k) M = fmaxf(M, sm[tid + k * per][0]);
+      const float Mu = (M == kNegInf) ? 0.f : M;
+      const float mine = exp2f(sm[tid][0] - Mu);
+      o *= mine;
+      l *= mine;
+      for (int k = 1; k < ngrp; ++k) {
+        const f32x2 x = sm[tid + k * per];
+        const float wt = exp2f(x[0] - Mu);
+        l += x[1] * wt;
+        o += so[tid + k * per] * wt;
+      }
+    }
+    if (on && d0 < p.dr) {
+      const float inv = (l == 0.f) ? 0.f : 1.f / l;  // no key, or none that weighs: o = 0
+      typedef T v4 __attribute__((ext_vector_type(4)));
+      v4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f32(o[e] * inv);
+      *reinterpret_cast<v4*>(static_cast<T*>(p.o) + bh * p.dr + d0) = y;
+    }
+  }
+}
+
+template <typename T, int D, bool DMA, int PG>
+hipError_t launch(const PrefixParams& p, hipStream_t st) {
+  const int own_wgs = PG > 0 ? (p.own.n_waves + 3) / 4 : p.own.n_waves;
+  const dim3 grid((unsigned)(p.n_pre + own_wgs));
+  if (grid.x > 0) {
+    hipLaunchKernelGGL((pf_prefix_kernel<T, D, DMA, PG>), grid, dim3(256), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D, (PG > 0 ? kOwnKeys : kBN)>),
+                     dim3((unsigned)(p.own.B * p.Hkv * ((p.g + 15) / 16))), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_pages(const PrefixParams& p, hipStream_t st) {
+  if (!p.dma) return launch<T, D, false, 0>(p, st);
+  if (!p.thin) return launch<T, D, true, 0>(p, st);
+  constexpr int PG = OwnGeo<T, D>::RPL == 8 ? 8 : 4;
+  return p.page_size % 16 == 0 ? launch<T, D, true, 16>(p, st) : launch<T, D, true, PG>(p, st);
+}
+
+template <typename T>
+hipError_t launch_dim(const PrefixParams& p, int D, hipStream_t st) {
+  if (D == 64) return launch_pages<T, 64>(p, st);
+  if (D == 128) return launch_pages<T, 128>(p, st);
+  if constexpr (sizeof(T) == 2)
+    if (D == 256) return launch_pages<T, 256>(p, st);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace prefix
+}  // namespace pf

@@ -874,24 +874,22 @@ int pf_paged_attn(const pf_paged_attn_args* a, void* stream) {
 // ---------------------------------------------------------------------------
 namespace {
 
-// The chunks. Prefix: one item per CU; own: enough items to go round, chunks of
-// 128 to 1024 keys.
+int own_waves(const pf::PrefixParams& p, bool thin) {
+  const int64_t keys = thin ? 16 : 64, most = thin ? 8 * kCus : 2 * kCus;
+  return (int)std::min(most, (int64_t)p.own.B * p.Hkv * p.n_hc * (((int64_t)p.own.pages_per_seq * p.page_size + keys - 1) / keys));
+}
+
+// The work: prefix chunks of at least 128 keys for an item per CU; the own keys
+// over at most two workgroups per CU, a wave (thin) or workgroup for as little as
+// one stage (by the longest lengths).
 void plan_prefix(pf::PrefixParams* p) {
-  const int64_t most = p->dma ? (int64_t)pf::kPrefixGroups << p->group_log2 : (int64_t)1 << 30;
-  auto chunk_of = [&](int64_t keys, int64_t pieces, int64_t lo, int64_t hi) {
-    const int64_t c = ((keys + pieces - 1) / pieces + 63) / 64 * 64;
-    return (int)std::min(most, std::min(hi, std::max(lo, c)));
-  };
-  const int64_t items = (int64_t)p->n_tiles * p->Hkv, seqs = (int64_t)p->B * p->Hkv * p->n_hc;
-  p->chunk = p->own_chunk = 64;
+  const int64_t items = (int64_t)p->n_tiles * p->Hkv;
   if (p->len > 0) {
-    p->chunk = chunk_of(p->len, std::max<int64_t>(1, kCus / items), 128, (int64_t)1 << 30);
+    const int64_t n = std::max<int64_t>(1, kCus / items);
+    p->chunk = (int)std::max<int64_t>(128, ((p->len + n - 1) / n + 63) / 64 * 64);
     p->n_split = (p->len + p->chunk - 1) / p->chunk;
   }
-  if (p->own_cap > 0) {
-    p->own_chunk = chunk_of(p->own_cap, std::max<int64_t>(1, 4 * kCus / seqs), 128, 1024);
-    p->n_own = (p->own_cap + p->own_chunk - 1) / p->own_chunk;
-  }
+  p->own.n_waves = own_waves(*p, p->thin);
 }
 
 // *D: the compute head dim.
@@ -906,15 +904,15 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   if (!dtype_ok(a->dtype)) return PF_ERR_UNSUPPORTED;
   if (!decode_head_dim_ok(a->head_dim, a->dtype)) return PF_ERR_UNSUPPORTED;
   *D = decode_compute_dim(a->head_dim);
-  const int64_t own_cap = (int64_t)a->pages_per_seq * a->page_size;
-  if (own_cap > kMaxGrid - 2048 || a->prefix_len > kMaxGrid - 2048) return PF_ERR_UNSUPPORTED;
-  if ((int64_t)a->batch * a->num_heads > kMaxGrid - 2 * pf::kPrefixRows) return PF_ERR_UNSUPPORTED;
+  // keys, rows and pool rows are counted in 32 bits
+  constexpr int64_t kMost = kMaxGrid - (1 << 20);
+  if ((int64_t)a->pages_per_seq * a->page_size > kMost || a->prefix_len > kMost) return PF_ERR_UNSUPPORTED;
+  if ((int64_t)a->batch * a->num_heads > kMost) return PF_ERR_UNSUPPORTED;
   *p = pf::PrefixParams{};
   p->q = a->q;
   p->k = a->k_pages;
   p->v = a->v_pages;
   p->o = a->o;
-  p->B = a->batch;
   p->Hq = a->num_heads;
   p->Hkv = a->num_kv_heads;
   p->g = a->num_heads / a->num_kv_heads;
@@ -922,32 +920,49 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   p->dr = a->head_dim;
   p->num_pages = a->num_pages;
   p->page_size = a->page_size;
+  p->div_page = pf::fast_divisor(a->page_size);
   p->scale_log2 = a->sm_scale * 1.4426950408889634f;
   p->table = a->prefix_table;
   p->len_ptr = a->prefix_len_ptr;
+  p->pages = a->prefix_pages;
   p->len = a->prefix_len;
   p->n_tiles = (p->rows + pf::kPrefixRows - 1) / pf::kPrefixRows;
-  p->own_tables = a->block_tables;
-  p->own_lens = a->context_lens;
-  p->pages_per_seq = a->pages_per_seq;
-  p->own_cap = (int)own_cap;
+  p->chunk = 64;
   p->n_hc = (p->g + pf::kPrefixRows - 1) / pf::kPrefixRows;
+  p->own_rows = std::min(p->g, pf::kPrefixRows);
+  p->own.B = a->batch;
+  p->own.block_tables = a->block_tables;
+  p->own.context_lens = a->context_lens;
+  p->own.page_size = a->page_size;
+  p->own.pages_per_seq = a->pages_per_seq;
   const int rows_per_load = 1024 / (*D * (a->dtype == PF_DTYPE_F32 ? 4 : 2));
-  while (p->group_log2 < 6 && a->page_size % (2 << p->group_log2) == 0) ++p->group_log2;
-  // pool rows are counted in 32 bits
   p->dma = a->page_size % rows_per_load == 0 &&
-           (int64_t)a->num_pages * a->page_size <= (int64_t)0xffffffff / a->num_kv_heads;
+           (int64_t)a->num_pages * a->page_size <= (int64_t)0xffffffff / a->num_kv_heads &&
+           (((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0;
+  // own_stream: at most 8 heads, whole rows of a kernel's head dim, whole page groups
+  p->thin = p->dma && p->g <= 8 && a->head_dim == *D && a->page_size % std::max(4, rows_per_load) == 0 &&
+            ((uintptr_t)a->q & 15) == 0;
   if (a->batch > 0) plan_prefix(p);
   const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
-  const int64_t n_own = (int64_t)p->B * p->Hkv * p->n_hc * p->n_own;
-  if (n_pre + n_own > kMaxGrid) return PF_ERR_UNSUPPORTED;
+  if (n_pre + p->own.n_waves > kMaxGrid) return PF_ERR_UNSUPPORTED;
   p->n_pre = (int)n_pre;
-  p->dma = p->dma && (((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0;
   return PF_OK;
 }
 
-size_t prefix_rows(const pf::PrefixParams& p) { return (size_t)(p.n_split + p.n_own) * p.B * p.Hq; }
-size_t prefix_ws(const pf::PrefixParams& p, int D) { return std::max<size_t>(partial_bytes(prefix_rows(p), D), 256); }
+// Rows of the partials: of the prefix's chunks, and of the own pieces (own_slot).
+size_t prefix_rows(const pf::PrefixParams& p) { return (size_t)p.n_split * p.own.B * p.Hq; }
+size_t form_piece_rows(const pf::PrefixParams& p, bool thin) {
+  const size_t seqs = (size_t)p.own.B * p.Hkv * p.n_hc, w = own_waves(p, thin);
+  return w == 0 ? 0 : (seqs + (seqs <= w ? 1 : 2) * w) * p.own_rows;
+}
+// The own pieces of either form, so that the size does not depend on how the pools
+// are aligned.
+size_t own_piece_rows(const pf::PrefixParams& p) {
+  return std::max(form_piece_rows(p, true), form_piece_rows(p, false));
+}
+size_t prefix_ws(const pf::PrefixParams& p, int D) {
+  return std::max<size_t>(partial_bytes(prefix_rows(p), D) + partial_bytes(own_piece_rows(p), D), 256);
+}
 
 }  // namespace
 
@@ -967,8 +982,12 @@ int pf_paged_prefix_attn(const pf_paged_prefix_attn_args* a, void* stream) {
   if ((a->pages_per_seq > 0 && !a->block_tables) || (a->prefix_len > 0 && !a->prefix_table)) return PF_ERR_INVALID;
   if (!a->workspace || a->workspace_bytes < prefix_ws(p, D) || ((uintptr_t)a->workspace & 255) != 0)
     return PF_ERR_WORKSPACE;
-  p.part_o = static_cast<float*>(a->workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + align256(prefix_rows(p) * D * sizeof(float)));
+  char* ws = static_cast<char*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + align256(prefix_rows(p) * D * sizeof(float)));
+  ws += partial_bytes(prefix_rows(p), D);
+  p.own.part_o = reinterpret_cast<float*>(ws);
+  p.own.part_ml = reinterpret_cast<float*>(ws + align256(own_piece_rows(p) * D * sizeof(float)));
   return finish(pf::launch_prefix(p, a->dtype, D, (hipStream_t)stream));
 }
 

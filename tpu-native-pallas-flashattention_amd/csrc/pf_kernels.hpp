@@ -112,6 +112,22 @@ __device__ inline SplitItem split_item(int bid, int n_blk, int members, F count)
   return SplitItem{0, 0, 0};  // not reached: bid < the grid, the sum of the counts
 }
 
+// n / d of n < 2^31 by a multiplier: with l = ceil(log2 d) and m =
+// floor(2^(31 + l) / d) + 1 <= 2^32, n m / 2^(31 + l) lies less than 1 / d above
+// n / d. (m = 2^32 for no d: a power of two has m = 2^31 + 1.)
+struct FastDiv {
+  uint32_t d, mul;
+  int shift;
+};
+__device__ inline uint32_t fast_div(uint32_t n, const FastDiv& f) {
+  return (uint32_t)(((uint64_t)n * f.mul) >> f.shift);
+}
+inline FastDiv fast_divisor(int d) {
+  int l = 0;
+  while (((int64_t)1 << l) < d) ++l;
+  return FastDiv{(uint32_t)d, (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)d) + 1), 31 + l};
+}
+
 // Forward prefill (optionally with fused RoPE).
 struct FwdParams {
   const void* q;
@@ -321,36 +337,47 @@ int decode_stream_qrows(int group);               // query rows per partial slot
 hipError_t launch_decode_stream(const DecodeParams& p, int dtype, bool paged, hipStream_t stream);
 
 // Attention of a batch over a shared prefix (attn_prefix.hip).
-constexpr int kPrefixRows = 128;     // query rows per workgroup
-constexpr int kPrefixGroups = 1024;  // page lookups a workgroup can hold
+constexpr int kPrefixRows = 128;  // query rows per workgroup
 struct PrefixParams {
   const void* q;  // [B, Hq, dr]
   const void* k;  // page pools
   const void* v;
   void* o;
-  int B, Hq, Hkv, g, rows;  // rows = B g
-  int dr;                   // stored head dim
+  int Hq, Hkv, g, rows;  // rows = B g
+  int dr;                // stored head dim
   int num_pages, page_size;
+  FastDiv div_page;
   int dma;         // whole loads lie inside a page and the pools are aligned
-  int group_log2;  // keys of one page lookup (a power of two that divides page_size, at most 64)
   float scale_log2;
-  // the prefix: chunks [0, n_split) of `chunk` keys (a multiple of 64)
-  const int32_t* table;
+  // the prefix
+  const int32_t* table;    // [pages]
   const int32_t* len_ptr;  // its length in device memory (at most len), or null: len
-  int len;
+  int pages, len;
   int n_tiles;             // ceil(rows / kPrefixRows)
-  int chunk, n_split;
+  int chunk, n_split;      // chunks of `chunk` keys (a multiple of 64)
   int n_pre;               // work items: n_tiles Hkv n_split
-  // the sequences' own keys: chunks [n_split, n_split + n_own)
-  const int32_t* own_tables;  // [B, pages_per_seq]
-  const int32_t* own_lens;    // [B]
-  int pages_per_seq, own_cap;  // own_cap = pages_per_seq page_size
-  int own_chunk, n_own;
-  int n_hc;                // ceil(g / kPrefixRows)
-  float* part_o;   // [n_split + n_own, B, Hq, D]
-  float* part_ml;  // [n_split + n_own, B, Hq, 2]
+  float* part_o;           // [n_split, B, Hq, D]
+  float* part_ml;          // [n_split, B, Hq, 2]
+  // The sequences' own keys: the streaming decode's work list. Of `own`: B,
+  // block_tables, context_lens, page_size, pages_per_seq, n_waves, and the
+  // partials, own_rows rows per slot. thin: in stages of 16 keys over n_waves
+  // waves (own_stream); else in blocks of 64 keys over n_waves workgroups.
+  DecodeParams own;
+  int thin;
+  int n_hc;      // ceil(g / kPrefixRows) slices of a KV head's query heads
+  int own_rows;  // min(g, kPrefixRows)
 };
-hipError_t launch_prefix(const PrefixParams& p, int dtype, int D, hipStream_t stream);
+hipError_t launch_prefix_f32(const PrefixParams& p, int D, hipStream_t stream);
+hipError_t launch_prefix_bf16(const PrefixParams& p, int D, hipStream_t stream);
+hipError_t launch_prefix_f16(const PrefixParams& p, int D, hipStream_t stream);
+inline hipError_t launch_prefix(const PrefixParams& p, int dtype, int D, hipStream_t stream) {
+  switch (dtype) {
+    case kF32: return launch_prefix_f32(p, D, stream);
+    case kBF16: return launch_prefix_bf16(p, D, stream);
+    case kF16: return launch_prefix_f16(p, D, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
 
 // Cache writes (cache_ops.hip). positions: device int32, read at
 // b * pos_stride (pos_stride 0 = one position for the whole batch).
@@ -383,10 +410,6 @@ hipError_t launch_paged_cache_write(const PagedWriteParams& p, int dtype, int he
 // Multi-axis rotation of q and k, or rotation of q and append of k and v to a
 // paged pool (rope_axes.hip).
 constexpr int kMaxRopeAxes = 4;
-struct FastDiv {
-  uint32_t d, mul;
-  int shift;
-};
 struct RopeAxesParams {
   const void* x[3];  // q, k, v: [B, heads, S, D], strides (elements) of the first three dimensions
   int64_t sb[3], sh[3], ss[3];

@@ -30,18 +30,6 @@ namespace pf {
 
 namespace {
 
-// n / d of n < 2^31 by the divisor's multiplier (fast_divisor): with l =
-// ceil(log2 d) and m = floor(2^(31 + l) / d) + 1 < 2^32, n m / 2^(31 + l) lies
-// less than 1 / d above n / d.
-__device__ inline uint32_t fast_div(uint32_t n, const FastDiv& f) {
-  return (uint32_t)(((uint64_t)n * f.mul) >> f.shift);
-}
-FastDiv fast_divisor(int d) {
-  int l = 0;
-  while (((int64_t)1 << l) < d) ++l;
-  return FastDiv{(uint32_t)d, (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)d) + 1), 31 + l};
-}
-
 // E elements, element-aligned: rows need no 16-byte alignment.
 template <typename T, int E>
 struct Vec {
