@@ -18,14 +18,24 @@
 // No counterpart in the reference, whose paged call gives the prefix's pages
 // to every sequence's table (paged.py:102-192).
 //
-// A prefix item runs the prefill forward's pipeline (attn_fwd.hip) over pages: K
-// one 64-key block ahead of V, both double-buffered in LDS; S^T = K Q^T runs
-// beside the exponentials of the block before, O^T += V^T P^T beside the maximum
-// of the block after. The tiles come by direct global -> LDS loads of whole rows
-// (1 KB each, inside one page; rows past the length and columns past the stored
-// head dim lie outside the load's buffer range and arrive as zeros); a block's
-// pages are looked up one block before its loads. Pages that such loads would
-// straddle and unaligned pools are staged through registers instead.
+// A prefix item runs the prefill forward's arithmetic (attn_fwd.hip) over pages:
+// 64-key blocks in LDS, S^T = K Q^T of block t + 1 beside the exponentials of
+// block t, O^T += V^T P^T of block t beside the maximum of block t + 1. Its keys
+// come from memory, not from an L2 that many workgroups share, and the own keys
+// beside it keep memory busy, so the loads run further ahead than there, in as
+// many tiles (two of K, two of V): a second barrier, in the middle of a block,
+// frees K_{t+1}'s tile for K_{t+3} while P.V of block t runs, and a wait is for the
+// tile needed next alone. The tiles come by direct global -> LDS loads of whole
+// rows (1 KB each, inside one page; rows past the length and columns past the
+// stored head dim lie outside the load's buffer range and arrive as zeros). Pages
+// that such loads would straddle and unaligned pools are staged through registers
+// instead.
+// Measured (bfloat16, head_dim 128, 32 heads over 8, 128 sequences, 32768 prefix
+// keys): the prefix alone 98 us, 702 TFLOP/s. One wave a SIMD leaves the pipeline
+// bound by its instructions; what helped was one lookup and descriptor per tile
+// (pages of 64 rows), tile addresses that are constants of each block's copy, and
+// nothing of the own keys' code in the loop. With the own keys (4.3 MB a sequence)
+// 144 us: 98 us of reads beside 98 us of products that share the SIMDs.
 //
 // Own keys with at most 8 heads a KV head: the workgroup's waves each stream a
 // run of their own (own_stream). More heads, stored head dims that are not a
@@ -63,59 +73,72 @@ __device__ inline int64_t own_slot(const DecodeParams& p, int J, int w, int64_t 
 }
 
 // Loads of 64-row tiles: the keys [64 st, ...) below L of the cursor's sequence.
-// DMA: each wave's loads are RPL whole rows of one page; else every lane fetches
-// its 16-byte chunks itself.
-template <typename T, int D, bool DMA>
+// DMA > 0: each wave's loads are whole rows of one page; 64: of a page that holds
+// the whole tile (page_size % 64 == 0), so that a tile takes one lookup and one
+// descriptor -- with a wave on each SIMD the scalar instructions of eight of them
+// cost as much as the exponentials. DMA = 0: every lane fetches its 16-byte chunks
+// itself.
+template <typename T, int D, int DMA>
 struct PageTiles {
   using G = Tile<T, D>;
-  static constexpr int PT = G::CPR / 4;         // loads per lane and tile
-  static constexpr int RPL = 1024 / G::RB;      // rows per load
-  uint32_t voff[PT];  // DMA: the lane's byte offset within the load's rows
-  uint32_t row0;      // DMA: the wave's first row of load 0; load u: + 4 RPL u
+  static constexpr int PT = G::CPR / 4;          // loads per lane and tile
+  static constexpr int RPL = 1024 / G::RB;       // rows per load
+  static constexpr int GR = DMA == 64 ? 64 : RPL;  // rows per lookup
+  static constexpr int NG = DMA == 64 ? 1 : PT;    // lookups of a wave per tile
+  uint32_t voff[PT];  // the lane's byte offset within the lookup's rows
+  uint32_t row0;      // the wave's first row of load 0; load u: + 4 RPL u
   uint32_t slot0;     // the wave's LDS byte offset of load 0; load u: + 4096 u
+  uint32_t rb;        // stored row bytes
   int lane, n_hc;
   const PrefixParams& p;
   const int32_t* table;  // of the prefix, or all sequences'
   int pages;             // per sequence
 
   __device__ inline PageTiles(const PrefixParams& p_, int tid, bool own)
-      : lane(tid & 63), n_hc(own ? p_.n_hc : 1), p(p_), table(own ? p_.own.block_tables : p_.table),
-        pages(own ? p_.own.pages_per_seq : p_.pages) {
+      : rb(p_.dr * G::ES), lane(tid & 63), n_hc(own ? p_.n_hc : 1), p(p_),
+        table(own ? p_.own.block_tables : p_.table), pages(own ? p_.own.pages_per_seq : p_.pages) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     row0 = RPL * w;
     slot0 = 1024 * w;
 #pragma unroll
     for (int u = 0; u < PT; ++u) {
-      const int r = lane / G::CPR, row = RPL * (4 * u + w) + r;
+      const int row = RPL * (4 * u + w) + lane / G::CPR, r = DMA == 64 ? row : lane / G::CPR;
       const int chunk = (lane % G::CPR) ^ tile_swz<G::CPR>(row);
       // columns past the stored row: past any range
       voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((r * p.dr + chunk * G::EPC) * G::ES) : 0x7ffffff0u;
     }
   }
   __device__ inline int kv_head(const Cursor& c) const { return n_hc == 1 ? c.j : c.j / n_hc; }
-  // The page lookups of the wave's loads of a block, load u in lane u: the
-  // entry, and where the load starts in the page. A load past the table's reach
-  // looks up the last page and reads nothing.
-  struct Look {
-    int page;
-    uint32_t off;
+  // The byte offsets in the pool where a block's lookups start (wave-uniform;
+  // scalar loads of the table, which do not disturb the count of the loads in
+  // flight), and the bytes behind them that are valid. A lookup past the table's
+  // reach takes the last page and reads nothing.
+  struct Rows {
+    uint64_t at[NG];
+    uint32_t bytes[NG];
   };
-  __device__ inline Look look(const Cursor& c) const {
-    const int key = kBN * c.st + row0 + 4 * RPL * (lane & (PT - 1));
-    const int lp = min((int)fast_div(key, p.div_page), pages - 1);
-    return Look{table[(int64_t)c.b * pages + lp], (uint32_t)(key - lp * p.page_size)};
+  __device__ inline Rows rows(const Cursor& c) const {
+    Rows x;
+    const int kvh = kv_head(c);
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const int key = kBN * c.st + (DMA == 64 ? 0 : row0 + 4 * RPL * u);
+      const int lp = min((int)fast_div(key, p.div_page), pages - 1);
+      const int page = min(max(stream::sload_i32(table, (int64_t)c.b * pages + lp), 0), p.num_pages - 1);
+      x.at[u] = (uint64_t)(((uint32_t)page * p.Hkv + kvh) * p.page_size + (key - lp * p.page_size)) * rb;
+      x.bytes[u] = min(max(c.L - key, 0), GR) * rb;
+    }
+    return x;
   }
-  // The pool rows where the loads start (in lane u), once the entries are there.
-  __device__ inline uint32_t rows(const Cursor& c, const Look& l) const {
-    const int page = min(max(l.page, 0), p.num_pages - 1);
-    return ((uint32_t)page * p.Hkv + kv_head(c)) * p.page_size + l.off;
+  // The descriptor of the whole tile (DMA = 64), for all its loads.
+  __device__ inline i32x4 tile_desc(const void* pool, const Rows& x) const {
+    return dma_pin(make_desc(static_cast<const char*>(pool) + x.at[0], x.bytes[0]));
   }
-  __device__ inline void load(const void* pool, const Cursor& c, uint32_t rows, int u, char* tile) const {
-    const int key = kBN * c.st + row0 + 4 * RPL * u;
-    const int valid = min(max(c.L - key, 0), RPL);
-    const uint32_t rb = p.dr * G::ES;
-    const uint32_t row = __builtin_amdgcn_readlane(rows, u);
-    const i32x4 d = make_desc(static_cast<const char*>(pool) + (uint64_t)row * rb, valid * rb);
+  __device__ inline void load(const i32x4& pinned, int u, char* tile) const {
+    dma16_pinned<true>(pinned, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 4096 * u));
+  }
+  __device__ inline void load(const void* pool, const Rows& x, int u, char* tile) const {
+    const i32x4 d = make_desc(static_cast<const char*>(pool) + x.at[u], x.bytes[u]);
     dma16<true>(d, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 4096 * u));
   }
   // Without DMA: a block through registers.
@@ -386,75 +409,172 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   }
 }
 
-// PG > 0: own keys by own_stream; 0: by the block pipeline.
-template <typename T, int D, bool DMA, int PG>
-__global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(PrefixParams p) {
+// The block pipeline of one workgroup: a prefix item, or (OWN) its run of the
+// sequences' own keys. item: the workgroup's place among those of its kind.
+template <typename T, int D, int DMA, bool OWN>
+__device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, int item) {
   using MF = Mfma32<T>;
   using Frag = typename MF::Frag;
   using G = Tile<T, D>;
   using PTiles = PageTiles<T, D, DMA>;
   constexpr int HALF = D / 2, EPC = G::EPC, FPC = frags_per_chunk<T>();
   constexpr int QF = HALF / MF::kK, NDT = D / 32, PF = 32 / MF::kK, PT = PTiles::PT;
-  // K blocks t & 1, then V blocks; or the waves' rings
-  static_assert(4 * OwnGeo<T, D>::WAVE >= 4 * G::BYTES, "the rings hold two blocks");
-  __shared__ __attribute__((aligned(1024))) char smem[PG > 0 ? 4 * OwnGeo<T, D>::WAVE : 4 * G::BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hh = lane >> 5, l32 = lane & 31;
-  const bool own_wg = blockIdx.x >= (unsigned)p.n_pre;
-  if constexpr (PG > 0) {
-    if (own_wg) {
-      own_stream<T, D, PG>(p, smem + wv * OwnGeo<T, D>::WAVE, 4 * (blockIdx.x - p.n_pre) + wv);
-      return;
-    }
-  }
-  const bool own = PG == 0 && own_wg;
   const int J = p.Hkv * p.n_hc;
 
   // The workgroup's n blocks and the first one's cursor.
   Cursor cp;
   int n, r0 = 0, piece = 0;
-  if (!own) {
+  if constexpr (!OWN) {
     // (chunk, kv head, row tile): the row tiles of one chunk side by side on one
     // XCD, whose L2 then serves the chunk to all of them.
-    const int item = xcd_remap(blockIdx.x, p.n_pre, p.n_tiles);
-    r0 = kRows * (item % p.n_tiles);
-    piece = item / p.n_tiles / p.Hkv;
+    const int it = xcd_remap(item, p.n_pre, p.n_tiles);
+    r0 = kRows * (it % p.n_tiles);
+    piece = it / p.n_tiles / p.Hkv;
     const int key0 = piece * p.chunk, L = min(prefix_len(p), key0 + p.chunk);
     n = (L - key0 + kBN - 1) / kBN;
-    cp = Cursor{0, item / p.n_tiles % p.Hkv, key0 / kBN, key0 / kBN + n, L};
+    cp = Cursor{0, it / p.n_tiles % p.Hkv, key0 / kBN, key0 / kBN + n, L};
   } else {
     stream::Partition part((int64_t)0, (int64_t)0);
-    n = (int)stream::wave_plan<kPG, kBN>(p.own, J, p.own.n_waves, blockIdx.x - p.n_pre, &cp, &part);
+    n = (int)stream::wave_plan<kPG, kBN>(p.own, J, p.own.n_waves, item, &cp, &part);
   }
+  n = __builtin_amdgcn_readfirstlane(n);  // barriers are counted by it
   if (n <= 0) return;
 
-  const PTiles tiles(p, tid, own);
-  char* const kbuf0 = smem;
-  char* const vbuf0 = smem + 2 * G::BYTES;
-  auto next = [&](Cursor& c) { stream::cursor_next<kPG, kBN>(c, p.own, J); };
+  const PTiles tiles(p, tid, OWN);
+  // The cursor of the block after c's (block t of the run); past the run, one whose
+  // loads read nothing: every block issues the same loads, so that the waits can
+  // count them.
+  auto after = [&](Cursor c, int t) {
+    if (t + 1 >= n) c.L = 0;
+    else if constexpr (OWN) stream::cursor_next<kPG, kBN>(c, p.own, J);
+    else ++c.st;
+    return c;
+  };
 
   // An own block seldom has rows for more than one wave: which one differs from
   // workgroup to workgroup, so that those on a CU load all of its SIMDs.
-  const int w32 = 32 * (own ? (wv + blockIdx.x) & 3 : wv);
+  const int w32 = 32 * (OWN ? (wv + item) & 3 : wv);
   // The lane's query row in the cursor's sequence: (batch, head) index, or -1.
   auto row_of = [&](const Cursor& c) -> int {
-    if (!own) {
+    if constexpr (!OWN) {
       const int r = r0 + w32 + l32;
       if (r >= p.rows) return -1;
       const int b = r / p.g;
       return b * p.Hq + c.j * p.g + (r - b * p.g);
+    } else {
+      const int kvh = tiles.kv_head(c), r = kRows * (c.j - kvh * p.n_hc) + w32 + l32;
+      return r < p.g ? c.b * p.Hq + kvh * p.g + r : -1;
     }
-    const int kvh = tiles.kv_head(c), r = kRows * (c.j - kvh * p.n_hc) + w32 + l32;
-    return r < p.g ? c.b * p.Hq + kvh * p.g + r : -1;
   };
-  // Whether the wave has rows at all: of an own sequence's slices only the last
-  // can be short, so a wave without rows there may have some in others.
-  const bool active = own ? w32 < p.own_rows : r0 + w32 < p.rows;
+
+  // Cursors of blocks t (cp) .. t + 3 (cl), and where the loads of blocks t + 1 ..
+  // t + 3 start.
+  char* const kbuf = smem;  // K tiles t & 1, then V tiles
+  char* const vbuf = smem + 2 * G::BYTES;
+  Cursor cs = after(cp, 0), ck = after(cs, 1), cl = after(ck, 2);
+  typename PTiles::Rows r1, r2, r3;
+  auto whole = [&](const void* pool, [[maybe_unused]] const Cursor& c, const typename PTiles::Rows& x, char* tile) {
+    if constexpr (DMA == 64) {
+      const i32x4 d = tiles.tile_desc(pool, x);
+#pragma unroll
+      for (int u = 0; u < PT; ++u) tiles.load(d, u, tile);
+    } else if constexpr (DMA > 0) {
+#pragma unroll
+      for (int u = 0; u < PT; ++u) tiles.load(pool, x, u, tile);
+    } else {
+      tiles.copy(pool, c, tile);
+    }
+  };
+  {
+    typename PTiles::Rows r;
+    if constexpr (DMA > 0) {
+      r = tiles.rows(cp);
+      r1 = tiles.rows(cs);
+      r2 = tiles.rows(ck);
+      r3 = tiles.rows(cl);
+    }
+    whole(p.k, cp, r, kbuf);
+    whole(p.k, cs, r1, kbuf + G::BYTES);
+    whole(p.v, cp, r, vbuf);
+  }
+  // Block t, P = t & 1 (the tiles' addresses are constants of each copy): V_{t+1},
+  // beside S_{t+1}, goes where V_{t-1} was, K_{t+3}, beside P.V, where K_{t+1} was.
+  auto kcur = [&](auto par) { return kbuf + (1 - decltype(par)::value) * G::BYTES; };
+  auto vcur = [&](auto par) { return vbuf + decltype(par)::value * G::BYTES; };
+  auto vdst = [&](auto par) { return vbuf + (1 - decltype(par)::value) * G::BYTES; };
+  i32x4 vd, kd;
+  auto begin = [&](auto par) __attribute__((always_inline)) {
+    if constexpr (DMA == 64) {
+      vd = tiles.tile_desc(p.v, r1);
+      kd = tiles.tile_desc(p.k, r3);
+    }
+    if constexpr (DMA == 0) tiles.copy(p.v, cs, vdst(par));
+  };
+  auto v_part = [&](int i, auto par) __attribute__((always_inline)) {
+    if constexpr (DMA == 64) tiles.load(vd, i, vdst(par));
+    else if constexpr (DMA > 0) tiles.load(p.v, r1, i, vdst(par));
+  };
+  auto k_part = [&](int i, auto par) __attribute__((always_inline)) {
+    if constexpr (DMA == 64) tiles.load(kd, i, kcur(par));
+    else if constexpr (DMA > 0) tiles.load(p.k, r3, i, kcur(par));
+  };
+  // The middle: V_t is there (after it K_{t+2} and V_{t+1} were asked for), and
+  // every wave is done with K_{t+1}.
+  auto middle = [&](auto par) __attribute__((always_inline)) {
+    wait_vm<2 * PT>();
+    __syncthreads();
+    if constexpr (DMA == 0) tiles.copy(p.k, cl, kcur(par));
+  };
+  auto end = [&](int t) __attribute__((always_inline)) {
+    cp = cs;
+    cs = ck;
+    ck = cl;
+    cl = after(cl, t + 3);
+    if constexpr (DMA > 0) {
+      r1 = r2;
+      r2 = r3;
+      r3 = tiles.rows(cl);
+    }
+    wait_vm<2 * PT>();  // K_{t+2}: V_{t+1} and K_{t+3} were asked for after it
+    __syncthreads();
+  };
+  auto all_blocks = [&](auto&& block) __attribute__((always_inline)) {
+    int t = 0;
+    for (; t + 2 < n; t += 2) {
+      block(t, std::integral_constant<int, 0>{});
+      block(t + 1, std::integral_constant<int, 1>{});
+    }
+    if (t + 1 < n) block(t, std::integral_constant<int, 0>{});
+  };
+
+  // A wave without rows loads its share, and meets the others' barriers. (Of an
+  // own sequence's slices only the last can be short.)
+  const bool active = __builtin_amdgcn_readfirstlane(OWN ? w32 < p.own_rows : r0 + w32 < p.rows) != 0;
+  if (!active) {
+    dma_wait();
+    __syncthreads();
+    __syncthreads();
+    whole(p.k, ck, r2, kbuf);
+    all_blocks([&](int t, auto par) __attribute__((always_inline)) {
+      begin(par);
+#pragma unroll
+      for (int i = 0; i < PT; ++i) v_part(i, par);
+      middle(par);
+#pragma unroll
+      for (int i = 0; i < PT; ++i) k_part(i, par);
+      end(t);
+    });
+    wait_vm<0>();
+    __syncthreads();
+    return;
+  }
 
   u32x4 qc[HALF / EPC];  // Q: the lane's row, columns [hh HALF, + HALF)
-  auto load_q = [&](const Cursor& c) {
+  auto load_q = [&](const Cursor& c) __attribute__((always_inline)) {
     const int r = row_of(c);
     const T* qr = static_cast<const T*>(p.q) + (int64_t)r * p.dr + hh * HALF;
 #pragma unroll
@@ -462,48 +582,19 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
       qc[i] = r >= 0 && hh * HALF + i * EPC < p.dr ? ldg16(qr + i * EPC) : (u32x4){0u, 0u, 0u, 0u};
   };
   // A negative scale is applied as |scale| on -Q.
-  auto sign_q = [&]() {
+  auto sign_q = [&]() __attribute__((always_inline)) {
     if (p.scale_log2 < 0.f) {
       const uint32_t sign = G::ES == 4 ? 0x80000000u : 0x80008000u;
 #pragma unroll
       for (int i = 0; i < HALF / EPC; ++i) qc[i] ^= (u32x4){sign, sign, sign, sign};
     }
   };
-  auto frags = [&](Frag* qf) {
+  auto frags = [&](Frag* qf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < HALF / EPC; ++i)
 #pragma unroll
       for (int f = 0; f < FPC; ++f) qf[i * FPC + f] = chunk_frag<T>(qc[i], f);
   };
-
-  // Cursors of blocks t (cp), t + 1 (cs), t + 2 (ck); rv, lk: the pool rows of
-  // block t + 1 and the lookups of block t + 2.
-  Cursor cs = cp, ck = cp;
-  if (n > 1) next(cs);
-  if (n > 2) {
-    ck = cs;
-    next(ck);
-  }
-  uint32_t rv = 0;
-  typename PTiles::Look lk{};
-  if constexpr (DMA) {
-    const typename PTiles::Look l0 = tiles.look(cp), l1 = tiles.look(cs);
-    lk = tiles.look(ck);
-    const uint32_t r0s = tiles.rows(cp, l0);
-    rv = tiles.rows(cs, l1);
-#pragma unroll
-    for (int u = 0; u < PT; ++u) tiles.load(p.k, cp, r0s, u, kbuf0);
-#pragma unroll
-    for (int u = 0; u < PT; ++u) tiles.load(p.v, cp, r0s, u, vbuf0);
-    if (n > 1) {
-#pragma unroll
-      for (int u = 0; u < PT; ++u) tiles.load(p.k, cs, rv, u, kbuf0 + G::BYTES);
-    }
-  } else {
-    tiles.copy(p.k, cp, kbuf0);
-    tiles.copy(p.v, cp, vbuf0);
-    if (n > 1) tiles.copy(p.k, cs, kbuf0 + G::BYTES);
-  }
   load_q(cp);
 
   // Running maximum (log2 units) from the lowest finite value: scores of -inf
@@ -518,7 +609,7 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
 
   // m_run moves when some row's maximum grows by more than 8: p <= 2^8, and the
   // rescaling is rare.
-  auto update_max = [&](float mx) {
+  auto update_max = [&](float mx) __attribute__((always_inline)) {
     const float m_cand = fmaxf(m_run, mx);
     if (__any(m_cand > m_run + 8.f)) {
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_cand);
@@ -529,7 +620,7 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
     }
   };
   // The lane's maximum of a block's scores; keys at or past L become -inf.
-  auto block_max = [&](f32x16* s, const Cursor& c) {
+  auto block_max = [&](f32x16* s, const Cursor& c) __attribute__((always_inline)) {
     const int rel = c.L - kBN * c.st - 32 * hh;
     float mx = kNegInf;
 #pragma unroll
@@ -541,165 +632,146 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
     return mx;
   };
   // The end of a chunk or piece: its partials, and a fresh state.
-  bool first_piece = true;
-  int piece_st0 = cp.st;
-  auto finish = [&](const Cursor& c) {
+  [[maybe_unused]] bool first_piece = true;
+  [[maybe_unused]] int piece_st0 = cp.st;
+  auto finish = [&](const Cursor& c) __attribute__((always_inline)) {
     const float l_tot = wave_xor32_sum(l_run);
     const int r = row_of(c);
     if (r >= 0) {
       float *po = p.part_o, *pm = p.part_ml;
       int64_t at = (int64_t)piece * p.own.B * p.Hq + r;
-      if (own) {
-        const int w = blockIdx.x - p.n_pre;
+      if constexpr (OWN) {
         const int64_t seq = (int64_t)c.b * J + c.j;
-        const bool whole = piece_st0 == 0 && c.st == c.nst - 1;
-        at = own_slot(p.own, J, w, seq, whole, !first_piece) * p.own_rows + w32 + l32;
+        const bool whole_seq = piece_st0 == 0 && c.st == c.nst - 1;
+        at = own_slot(p.own, J, item, seq, whole_seq, !first_piece) * p.own_rows + w32 + l32;
         po = p.own.part_o;
         pm = p.own.part_ml;
       }
       store_acc_row<float, D>(po + at * D, acc, 1.f, hh);
       if (hh == 0) *reinterpret_cast<f32x2*>(pm + 2 * at) = (f32x2){m_run, l_tot};
     }
-    first_piece = false;
-    piece_st0 = 0;
-    m_run = -__FLT_MAX__;
-    l_run = 0.f;
+    if constexpr (OWN) {
+      first_piece = false;
+      piece_st0 = 0;
+      m_run = -__FLT_MAX__;
+      l_run = 0.f;
 #pragma unroll
-    for (int i = 0; i < NDT; ++i) acc[i] = (f32x16)(0.f);
+      for (int i = 0; i < NDT; ++i) acc[i] = (f32x16)(0.f);
+    }
   };
 
   dma_wait();
   __syncthreads();
   f32x16 s_cur[2] = {(f32x16)(0.f), (f32x16)(0.f)};
-  float mx_carry = kNegInf;  // the lane's maximum of the latest block, not yet applied
-  if (active) {
+  // The lane's maximum of the latest block, not yet applied. A block that the
+  // length cuts is masked when it is the run's last (before its exponentials), and
+  // at a sequence's end (OWN).
+  float mx_carry;
+  {
     sign_q();
     Frag qf[QF];
     frags(qf);
-    mfma_nat<T, D>(kbuf0, l32, hh, qf, s_cur[0], s_cur[1]);
+    mfma_nat<T, D>(kbuf, l32, hh, qf, s_cur[0], s_cur[1]);
     mx_carry = block_max(s_cur, cp);
-    if (own && n > 1 && cs.st == 0) {
+    if (OWN && n > 1 && cs.st == 0) {
       load_q(cs);
       sign_q();
     }
   }
   __syncthreads();  // K_0 is read before K_2 overwrites it
+  whole(p.k, ck, r2, kbuf);
 
-  for (int t = 0; t + 1 < n; ++t) {
-    char* const kcur = kbuf0 + ((t + 1) & 1) * G::BYTES;  // K_{t+1}
-    char* const vcur = vbuf0 + (t & 1) * G::BYTES;        // V_t
-    char* const kdst = kbuf0 + (t & 1) * G::BYTES;        // K_{t+2}
-    char* const vdst = vbuf0 + ((t + 1) & 1) * G::BYTES;  // V_{t+1}
-    const bool k_next = t + 2 < n;
-    Cursor cl = ck;  // block t + 3
-    if (t + 3 < n) next(cl);
-    uint32_t rk = 0;
-    auto load_part = [&](int i) __attribute__((always_inline)) {
-      if constexpr (DMA) {
-        if (i < PT) {
-          if (k_next) tiles.load(p.k, ck, rk, i, kdst);
-        } else if (i < 2 * PT) {
-          tiles.load(p.v, cs, rv, i - PT, vdst);
+  all_blocks([&](int t, auto par) __attribute__((always_inline)) {
+    const bool new_q = OWN && t + 2 < n && ck.st == 0;  // block t + 2 opens a sequence
+    f32x16 s_nxt[2] = {(f32x16)(0.f), (f32x16)(0.f)};
+    Frag qf[QF], pfr[PF];
+    frags(qf);
+    begin(par);
+    if constexpr (sizeof(T) == 2) {
+      // As in the forward: S_{t+1} beside the maximum and the first quarter of
+      // S_t's exponentials, P.V beside the rest.
+      constexpr int NV1 = G::CPR, NV2 = 4 * NDT, VPS2 = 32 / NV2;
+      uint32_t pw[16];
+      float rs = 0.f, mxr = kNegInf, mx = kNegInf;
+      auto exp_pair = [&](int pr) __attribute__((always_inline)) {
+        const int v = 2 * pr;
+        const float x0 = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
+        const float x1 = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][(v & 15) + 1], c2, -m_run));
+        pw[pr] = pack2<T>(x0, x1);  // the matrix cores take P in T: half a step of each weight
+        rs += x0 + x1;              // the sum is of the unrounded weights
+        asm volatile("" : "+v"(rs));  // keeps the sum beside its MFMA
+      };
+      mfma_nat_il<T, D>(kcur(par), l32, hh, qf, s_nxt[0], s_nxt[1], [&](int i) {
+        if (i < PT) v_part(i, par);
+        if (i == 0) {
+          mxr = wave_xor32_max(mx_carry) * c2;
+        } else if (i == 1) {
+          update_max(mxr);
+        } else {
+#pragma unroll
+          for (int pr = ((i - 2) * 4) / (NV1 - 2); pr < ((i - 1) * 4) / (NV1 - 2); ++pr) exp_pair(pr);
         }
-      }
-    };
-    if constexpr (DMA) {
-      rk = tiles.rows(ck, lk);
-      lk = tiles.look(cl);
-    } else {
-      if (k_next) tiles.copy(p.k, ck, kdst);
-      tiles.copy(p.v, cs, vdst);
-    }
-    const bool new_q = own && k_next && ck.st == 0;  // block t + 2 opens a sequence
-    if (!active) {
+      });
+      if (new_q) load_q(ck);  // Q is free now; there by the end of the block
+      middle(par);
+      pfr[0] = __builtin_bit_cast(Frag, (u32x4){pw[0], pw[1], pw[2], pw[3]});
+      mfma_trn_il<T, D>(vcur(par), vta, pfr, acc, [&](int i) {
+        if (i < PT) k_part(i, par);
 #pragma unroll
-      for (int i = 0; i < 2 * PT; ++i) load_part(i);
-    } else {
-      f32x16 s_nxt[2] = {(f32x16)(0.f), (f32x16)(0.f)};
-      Frag qf[QF], pfr[PF];
-      frags(qf);
-      const bool masked = (cs.st + 1) * kBN > cs.L;
-      if constexpr (sizeof(T) == 2) {
-        // As in the forward: S_{t+1} beside the maximum and the first quarter of
-        // S_t's exponentials, P.V beside the rest.
-        constexpr int NV1 = G::CPR, NV2 = 4 * NDT, VPS2 = 32 / NV2;
-        uint32_t pw[16];
-        float rs = 0.f, mxr = kNegInf, mx = kNegInf;
-        auto exp_pair = [&](int pr) __attribute__((always_inline)) {
-          const int v = 2 * pr;
-          const float x0 = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
-          const float x1 = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][(v & 15) + 1], c2, -m_run));
-          pw[pr] = pack2<T>(x0, x1);  // the matrix cores take P in T: half a step of each weight
-          rs += x0 + x1;              // the sum is of the unrounded weights
-          asm volatile("" : "+v"(rs));  // keeps the sum beside its MFMA
-        };
-        mfma_nat_il<T, D>(kcur, l32, hh, qf, s_nxt[0], s_nxt[1], [&](int i) {
-          load_part(i);
-          if (i == 0) {
-            mxr = wave_xor32_max(mx_carry) * c2;
-          } else if (i == 1) {
-            update_max(mxr);
-          } else {
-#pragma unroll
-            for (int pr = ((i - 2) * 4) / (NV1 - 2); pr < ((i - 1) * 4) / (NV1 - 2); ++pr) exp_pair(pr);
+        for (int pr = 4; pr < 16; ++pr) {
+          const int f = pr >> 2, q4 = pr & 3;
+          if (i == (f - 1) * NDT + (q4 * NDT) / 4) {
+            exp_pair(pr);
+            if (q4 == 3)
+              pfr[f] = __builtin_bit_cast(Frag, (u32x4){pw[4 * f], pw[4 * f + 1], pw[4 * f + 2], pw[4 * f + 3]});
           }
-        });
-        if (new_q) load_q(ck);  // Q is free now; there by the end of the block
-        pfr[0] = __builtin_bit_cast(Frag, (u32x4){pw[0], pw[1], pw[2], pw[3]});
-        mfma_trn_il<T, D>(vcur, vta, pfr, acc, [&](int i) {
-#pragma unroll
-          for (int pr = 4; pr < 16; ++pr) {
-            const int f = pr >> 2, q4 = pr & 3;
-            if (i == (f - 1) * NDT + (q4 * NDT) / 4) {
-              exp_pair(pr);
-              if (q4 == 3)
-                pfr[f] = __builtin_bit_cast(Frag, (u32x4){pw[4 * f], pw[4 * f + 1], pw[4 * f + 2], pw[4 * f + 3]});
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < VPS2; ++e) {
-            const int v = i * VPS2 + e;
-            mx = fmaxf(mx, s_nxt[v >> 4][v & 15]);
-          }
-          asm volatile("" : "+v"(mx));
-        });
-        l_run += rs;
-        mx_carry = mx;
-        if (masked) mx_carry = block_max(s_nxt, cs);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2 * PT; ++i) load_part(i);
-        __builtin_amdgcn_sched_barrier(0);
-        update_max(wave_xor32_max(mx_carry) * c2);
-        mfma_nat<T, D>(kcur, l32, hh, qf, s_nxt[0], s_nxt[1]);
-        if (new_q) load_q(ck);
-        float rs = 0.f;
-#pragma unroll
-        for (int v = 0; v < 32; ++v) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
-          s_cur[v >> 4][v & 15] = x;
-          rs += x;
         }
-        l_run += rs;
-        pack_frags<T>(s_cur[0], s_cur[1], pfr);
-        mfma_trn<T, D>(vcur, lane, vta, pfr, acc);
-        mx_carry = block_max(s_nxt, cs);
+#pragma unroll
+        for (int e = 0; e < VPS2; ++e) {
+          const int v = i * VPS2 + e;
+          mx = fmaxf(mx, s_nxt[v >> 4][v & 15]);
+        }
+        asm volatile("" : "+v"(mx));
+      });
+      l_run += rs;
+      mx_carry = mx;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PT; ++i) v_part(i, par);
+      __builtin_amdgcn_sched_barrier(0);
+      update_max(wave_xor32_max(mx_carry) * c2);
+      mfma_nat<T, D>(kcur(par), l32, hh, qf, s_nxt[0], s_nxt[1]);
+      if (new_q) load_q(ck);
+      float rs = 0.f, mx = kNegInf;
+#pragma unroll
+      for (int v = 0; v < 32; ++v) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s_cur[v >> 4][v & 15], c2, -m_run));
+        s_cur[v >> 4][v & 15] = x;
+        rs += x;
       }
-      s_cur[0] = s_nxt[0];
-      s_cur[1] = s_nxt[1];
-      if (own && cp.st == cp.nst - 1) finish(cp);
+      l_run += rs;
+      pack_frags<T>(s_cur[0], s_cur[1], pfr);
+      middle(par);
+#pragma unroll
+      for (int i = 0; i < PT; ++i) k_part(i, par);
+      mfma_trn<T, D>(vcur(par), lane, vta, pfr, acc);
+#pragma unroll
+      for (int v = 0; v < 32; ++v) mx = fmaxf(mx, s_nxt[v >> 4][v & 15]);
+      mx_carry = mx;
     }
-    dma_wait();
-    if (new_q && active) sign_q();
-    __syncthreads();
-    cp = cs;
-    cs = ck;
-    ck = cl;
-    rv = rk;
-  }
-  if (!active) return;
+    if constexpr (OWN) {
+      if ((cs.st + 1) * kBN > cs.L) mx_carry = block_max(s_nxt, cs);
+      if (cp.st == cp.nst - 1) finish(cp);
+      if (new_q) sign_q();
+    }
+    s_cur[0] = s_nxt[0];
+    s_cur[1] = s_nxt[1];
+    end(t);
+  });
+  wait_vm<0>();
+  __syncthreads();
 
-  update_max(wave_xor32_max(mx_carry) * c2);
+  update_max(wave_xor32_max(block_max(s_cur, cp)) * c2);
   {
     Frag pfr[PF];
     float rs = 0.f;
@@ -711,9 +783,28 @@ __global__ __launch_bounds__(256, (kFwdWgPerCu<T, D>)) void pf_prefix_kernel(Pre
     }
     l_run += rs;
     pack_frags<T>(s_cur[0], s_cur[1], pfr);
-    mfma_trn<T, D>(vbuf0 + ((n - 1) & 1) * G::BYTES, lane, vta, pfr, acc);
+    mfma_trn<T, D>(vbuf + ((n - 1) & 1) * G::BYTES, lane, vta, pfr, acc);
   }
   finish(cp);
+}
+
+// PG > 0: own keys by own_stream; 0: by the block pipeline.
+// The own pipeline needs the registers of two workgroups per CU at most.
+template <typename T, int D, int DMA, int PG>
+__global__ __launch_bounds__(256, (PG == 0 && kFwdWgPerCu<T, D> > 2 ? 2 : kFwdWgPerCu<T, D>))
+void pf_prefix_kernel(PrefixParams p) {
+  using G = OwnGeo<T, D>;
+  static_assert(4 * G::WAVE >= 4 * Tile<T, D>::BYTES, "the waves' rings hold the tiles");
+  __shared__ __attribute__((aligned(1024))) char smem[PG > 0 ? 4 * G::WAVE : 4 * Tile<T, D>::BYTES];
+  const int item = blockIdx.x - p.n_pre;
+  if (item < 0) {
+    run_blocks<T, D, DMA, false>(p, smem, blockIdx.x);
+  } else if constexpr (PG > 0) {
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    own_stream<T, D, PG>(p, smem + wv * G::WAVE, 4 * item + wv);
+  } else {
+    run_blocks<T, D, DMA, true>(p, smem, item);
+  }
 }
 
 // The merge: a workgroup per (batch, kv head, 16 of its heads), D / 4 lanes a
@@ -834,7 +925,7 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
   }
 }
 
-template <typename T, int D, bool DMA, int PG>
+template <typename T, int D, int DMA, int PG>
 hipError_t launch(const PrefixParams& p, hipStream_t st) {
   const int own_wgs = PG > 0 ? (p.own.n_waves + 3) / 4 : p.own.n_waves;
   const dim3 grid((unsigned)(p.n_pre + own_wgs));
@@ -850,10 +941,11 @@ hipError_t launch(const PrefixParams& p, hipStream_t st) {
 
 template <typename T, int D>
 hipError_t launch_pages(const PrefixParams& p, hipStream_t st) {
-  if (!p.dma) return launch<T, D, false, 0>(p, st);
-  if (!p.thin) return launch<T, D, true, 0>(p, st);
+  if (!p.dma) return launch<T, D, 0, 0>(p, st);
+  if (!p.thin) return launch<T, D, 1, 0>(p, st);
   constexpr int PG = OwnGeo<T, D>::RPL == 8 ? 8 : 4;
-  return p.page_size % 16 == 0 ? launch<T, D, true, 16>(p, st) : launch<T, D, true, PG>(p, st);
+  if (p.page_size % 64 == 0) return launch<T, D, 64, 16>(p, st);
+  return p.page_size % 16 == 0 ? launch<T, D, 1, 16>(p, st) : launch<T, D, 1, PG>(p, st);
 }
 
 template <typename T>

@@ -875,12 +875,13 @@ int pf_paged_attn(const pf_paged_attn_args* a, void* stream) {
 namespace {
 
 int own_waves(const pf::PrefixParams& p, bool thin) {
-  const int64_t keys = thin ? 16 : 64, most = thin ? 8 * kCus : 2 * kCus;
+  const int64_t keys = thin ? 16 : 64, most = thin ? 4 * kCus : kCus;
   return (int)std::min(most, (int64_t)p.own.B * p.Hkv * p.n_hc * (((int64_t)p.own.pages_per_seq * p.page_size + keys - 1) / keys));
 }
 
 // The work: prefix chunks of at least 128 keys for an item per CU; the own keys
-// over at most two workgroups per CU, a wave (thin) or workgroup for as little as
+// over at most one workgroup per CU (two: 39 us for 34, 64
+// sequences over 2000 prefix keys), a wave (thin) or workgroup for as little as
 // one stage (by the longest lengths).
 void plan_prefix(pf::PrefixParams* p) {
   const int64_t items = (int64_t)p->n_tiles * p->Hkv;
