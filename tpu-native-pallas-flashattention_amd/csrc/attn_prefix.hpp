@@ -33,7 +33,7 @@
 // Measured (bfloat16, head_dim 128, 32 heads over 8, 128 sequences, 32768 prefix
 // keys): the prefix alone 98 us, 702 TFLOP/s. One wave a SIMD leaves the pipeline
 // bound by its instructions; what helped was one lookup and descriptor per tile
-// (pages of 64 rows), tile addresses that are constants of each block's copy, and
+// and wave, tile addresses that are constants of each block's copy, and
 // nothing of the own keys' code in the loop. With the own keys (4.3 MB a sequence)
 // 144 us: 98 us of reads beside 98 us of products that share the SIMDs.
 //
@@ -73,21 +73,21 @@ __device__ inline int64_t own_slot(const DecodeParams& p, int J, int w, int64_t 
 }
 
 // Loads of 64-row tiles: the keys [64 st, ...) below L of the cursor's sequence.
-// DMA > 0: each wave's loads are whole rows of one page; 64: of a page that holds
-// the whole tile (page_size % 64 == 0), so that a tile takes one lookup and one
-// descriptor -- with a wave on each SIMD the scalar instructions of eight of them
-// cost as much as the exponentials. DMA = 0: every lane fetches its 16-byte chunks
-// itself.
+// Wave w loads rows 16 w .. 16 w + 15. DMA > 0: whole rows by direct loads; 16:
+// the wave's rows lie in one page (page_size % 16 == 0), so that a tile takes one
+// lookup and one descriptor -- with a wave on each SIMD the scalar instructions of
+// one per load cost as much as the exponentials; 1: each load's rows do. DMA = 0:
+// every lane fetches its 16-byte chunks itself.
 template <typename T, int D, int DMA>
 struct PageTiles {
   using G = Tile<T, D>;
   static constexpr int PT = G::CPR / 4;          // loads per lane and tile
   static constexpr int RPL = 1024 / G::RB;       // rows per load
-  static constexpr int GR = DMA == 64 ? 64 : RPL;  // rows per lookup
-  static constexpr int NG = DMA == 64 ? 1 : PT;    // lookups of a wave per tile
+  static constexpr int GR = DMA == 16 ? 16 : RPL;  // rows per lookup
+  static constexpr int NG = 16 / GR;             // lookups of a wave per tile
   uint32_t voff[PT];  // the lane's byte offset within the lookup's rows
-  uint32_t row0;      // the wave's first row of load 0; load u: + 4 RPL u
-  uint32_t slot0;     // the wave's LDS byte offset of load 0; load u: + 4096 u
+  uint32_t row0;      // the wave's first row; load u: + RPL u
+  uint32_t slot0;     // the wave's LDS byte offset of load 0; load u: + 1024 u
   uint32_t rb;        // stored row bytes
   int lane, n_hc;
   const PrefixParams& p;
@@ -98,14 +98,14 @@ struct PageTiles {
       : rb(p_.dr * G::ES), lane(tid & 63), n_hc(own ? p_.n_hc : 1), p(p_),
         table(own ? p_.own.block_tables : p_.table), pages(own ? p_.own.pages_per_seq : p_.pages) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    row0 = RPL * w;
-    slot0 = 1024 * w;
+    row0 = 16 * w;
+    slot0 = 1024 * PT * w;
 #pragma unroll
     for (int u = 0; u < PT; ++u) {
-      const int row = RPL * (4 * u + w) + lane / G::CPR, r = DMA == 64 ? row : lane / G::CPR;
-      const int chunk = (lane % G::CPR) ^ tile_swz<G::CPR>(row);
+      const int row = RPL * u + lane / G::CPR;
+      const int chunk = (lane % G::CPR) ^ tile_swz<G::CPR>(16 * w + row);
       // columns past the stored row: past any range
-      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((r * p.dr + chunk * G::EPC) * G::ES) : 0x7ffffff0u;
+      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((row % GR * p.dr + chunk * G::EPC) * G::ES) : 0x7ffffff0u;
     }
   }
   __device__ inline int kv_head(const Cursor& c) const { return n_hc == 1 ? c.j : c.j / n_hc; }
@@ -122,7 +122,7 @@ struct PageTiles {
     const int kvh = kv_head(c);
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
-      const int key = kBN * c.st + (DMA == 64 ? 0 : row0 + 4 * RPL * u);
+      const int key = kBN * c.st + row0 + GR * u;
       const int lp = min((int)fast_div(key, p.div_page), pages - 1);
       const int page = min(max(stream::sload_i32(table, (int64_t)c.b * pages + lp), 0), p.num_pages - 1);
       x.at[u] = (uint64_t)(((uint32_t)page * p.Hkv + kvh) * p.page_size + (key - lp * p.page_size)) * rb;
@@ -130,23 +130,23 @@ struct PageTiles {
     }
     return x;
   }
-  // The descriptor of the whole tile (DMA = 64), for all its loads.
-  __device__ inline i32x4 tile_desc(const void* pool, const Rows& x) const {
+  // The descriptor of the wave's rows (DMA = 16), for all its loads.
+  __device__ inline i32x4 rows_desc(const void* pool, const Rows& x) const {
     return dma_pin(make_desc(static_cast<const char*>(pool) + x.at[0], x.bytes[0]));
   }
   __device__ inline void load(const i32x4& pinned, int u, char* tile) const {
-    dma16_pinned<true>(pinned, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 4096 * u));
+    dma16_pinned<true>(pinned, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 1024 * u));
   }
   __device__ inline void load(const void* pool, const Rows& x, int u, char* tile) const {
     const i32x4 d = make_desc(static_cast<const char*>(pool) + x.at[u], x.bytes[u]);
-    dma16<true>(d, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 4096 * u));
+    dma16<true>(d, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 1024 * u));
   }
   // Without DMA: a block through registers.
   __device__ inline void copy(const void* pool, const Cursor& c, char* tile) const {
     u32x4 x[PT];
 #pragma unroll
     for (int u = 0; u < PT; ++u) {
-      const int s = (slot0 + 4096 * u) / 16 + lane, row = s / G::CPR;
+      const int s = (slot0 + 1024 * u) / 16 + lane, row = s / G::CPR;
       const int chunk = (s % G::CPR) ^ tile_swz<G::CPR>(row), key = kBN * c.st + row;
       x[u] = (u32x4){0u, 0u, 0u, 0u};
       if (key < c.L && chunk * G::EPC < p.dr) {
@@ -157,7 +157,7 @@ struct PageTiles {
       }
     }
 #pragma unroll
-    for (int u = 0; u < PT; ++u) sts16(tile + slot0 + 4096 * u + 16 * lane, x[u]);
+    for (int u = 0; u < PT; ++u) sts16(tile + slot0 + 1024 * u + 16 * lane, x[u]);
   }
 };
 
@@ -478,8 +478,8 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   Cursor cs = after(cp, 0), ck = after(cs, 1), cl = after(ck, 2);
   typename PTiles::Rows r1, r2, r3;
   auto whole = [&](const void* pool, [[maybe_unused]] const Cursor& c, const typename PTiles::Rows& x, char* tile) {
-    if constexpr (DMA == 64) {
-      const i32x4 d = tiles.tile_desc(pool, x);
+    if constexpr (DMA == 16) {
+      const i32x4 d = tiles.rows_desc(pool, x);
 #pragma unroll
       for (int u = 0; u < PT; ++u) tiles.load(d, u, tile);
     } else if constexpr (DMA > 0) {
@@ -508,18 +508,18 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   auto vdst = [&](auto par) { return vbuf + (1 - decltype(par)::value) * G::BYTES; };
   i32x4 vd, kd;
   auto begin = [&](auto par) __attribute__((always_inline)) {
-    if constexpr (DMA == 64) {
-      vd = tiles.tile_desc(p.v, r1);
-      kd = tiles.tile_desc(p.k, r3);
+    if constexpr (DMA == 16) {
+      vd = tiles.rows_desc(p.v, r1);
+      kd = tiles.rows_desc(p.k, r3);
     }
     if constexpr (DMA == 0) tiles.copy(p.v, cs, vdst(par));
   };
   auto v_part = [&](int i, auto par) __attribute__((always_inline)) {
-    if constexpr (DMA == 64) tiles.load(vd, i, vdst(par));
+    if constexpr (DMA == 16) tiles.load(vd, i, vdst(par));
     else if constexpr (DMA > 0) tiles.load(p.v, r1, i, vdst(par));
   };
   auto k_part = [&](int i, auto par) __attribute__((always_inline)) {
-    if constexpr (DMA == 64) tiles.load(kd, i, kcur(par));
+    if constexpr (DMA == 16) tiles.load(kd, i, kcur(par));
     else if constexpr (DMA > 0) tiles.load(p.k, r3, i, kcur(par));
   };
   // The middle: V_t is there (after it K_{t+2} and V_{t+1} were asked for), and
@@ -807,121 +807,119 @@ void pf_prefix_kernel(PrefixParams p) {
   }
 }
 
-// The merge: a workgroup per (batch, kv head, 16 of its heads), D / 4 lanes a
-// row, 16 bytes each; where the rows leave lanes over, groups of lanes share the
-// chunks and pieces and join through LDS. One wave finds the sequence's pieces in
-// the work list. Bound by the partials' latency: 8 are in flight per lane.
+// The merge: a workgroup per (batch, kv head, merge_heads of its heads), D / 4
+// lanes a row, 16 bytes each; groups of lanes share the chunks and pieces and join
+// through LDS. Bound by latency: the chunks' partials, 8 in flight per lane, are on
+// their way while each wave finds the sequence's pieces in the work list.
+// merge_heads is such that the chunks are one round of loads, where it can be.
+// ---------------------------------------------------------------------------
 template <typename T, int D, int SK>
 __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
-  constexpr int LPR = D / 4, NB = 8;
-  const int g = p.g, n16 = (g + 15) >> 4;
-  const int b = blockIdx.x / (p.Hkv * n16), j16 = blockIdx.x - b * p.Hkv * n16;
-  const int kvh = j16 / n16, h0 = 16 * (j16 - kvh * n16);  // heads [h0, + nq) of the group
-  const int nq = min(16, g - h0);
+  constexpr int LPR = D / 4, NB = kMergeLoads;
+  const int g = p.g, nh = p.merge_heads, n_h = (g + nh - 1) / nh;
+  const int b = blockIdx.x / (p.Hkv * n_h), jh = blockIdx.x - b * p.Hkv * n_h;
+  const int kvh = jh / n_h, h0 = nh * (jh - kvh * n_h);  // heads [h0, + nq) of the group
+  const int nq = min(nh, g - h0);
   const int tid = threadIdx.x;
+  const int per = nq * LPR, ngrp = 256 / per;  // per <= 256
+  const int grp = tid / per, i = tid - grp * per, qi = i / LPR, d0 = 4 * (i - LPR * qi);
+  const bool on = grp < ngrp;
+
+  float M = kNegInf, l = 0.f;
+  f32x4 o = (f32x4)(0.f);
+  f32x2 ml[NB];
+  f32x4 v[NB];
+  // Partials grp, grp + ngrp, ... of [s0, total): row(s) of po and pm.
+  auto fetch = [&](int s0, int total, const float* po, const float* pm, auto&& row) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NB; ++c) {
+      const int s = s0 + grp + c * ngrp;
+      ml[c] = (f32x2){kNegInf, 0.f};
+      v[c] = (f32x4)(0.f);
+      if (on && s < total) {
+        const int64_t r = row(s);
+        ml[c] = *reinterpret_cast<const f32x2*>(pm + r * 2);
+        v[c] = *reinterpret_cast<const f32x4*>(po + r * D + d0);
+      }
+    }
+  };
+  auto join = [&]() __attribute__((always_inline)) {
+    float Mn = M;
+#pragma unroll
+    for (int c = 0; c < NB; ++c) Mn = fmaxf(Mn, ml[c][0]);
+    const float Mu = (Mn == kNegInf) ? 0.f : Mn;
+    const float back = exp2f(M - Mu);
+    o *= back;
+    l *= back;
+#pragma unroll
+    for (int c = 0; c < NB; ++c) {
+      const float wt = exp2f(ml[c][0] - Mu);
+      l += ml[c][1] * wt;
+      o += v[c] * wt;
+    }
+    M = Mn;
+  };
+
+  const int npre = (prefix_len(p) + p.chunk - 1) / p.chunk;
+  const int64_t bh = (int64_t)b * p.Hq + kvh * g + h0 + qi;
+  auto chunk_row = [&](int s) { return (int64_t)s * p.own.B * p.Hq + bh; };
+  fetch(0, npre, p.part_o, p.part_ml, chunk_row);
+
+  // The sequence's np pieces: of wa and the workgroups (waves) after it.
   const int J = p.Hkv * p.n_hc, slice = h0 / kRows;
   const int64_t seq = (int64_t)b * J + kvh * p.n_hc + slice;
-
-  __shared__ int found[3];  // own pieces, first workgroup, whether it starts inside that one's run
-  if (tid < 64) {
-    int np = 0, wa = 0;
-    bool late = false;
-    if (p.own.n_waves > 0) {
-      const stream::BatchScan sc = stream::batch_scan<kPG, SK>(p.own, J);
-      const int L = sc.per == 1 ? __builtin_amdgcn_readlane(sc.L, b) : stream::seq_len<kPG>(p.own, b);
-      const int nst = (L + SK - 1) / SK;
-      if (nst > 0) {
-        const stream::Partition part(sc.tot, p.own.n_waves);
-        const int64_t s0 = stream::stages_before<kPG, SK>(p.own, J, b, sc) + (seq - (int64_t)b * J) * nst;
-        wa = part.wave_of(s0);
-        np = part.wave_of(s0 + nst - 1) - wa + 1;
-        late = part.start(wa) < s0;
-      }
-    }
-    if (tid == 0) {
-      found[0] = np;
-      found[1] = wa;
-      found[2] = late;
+  int np = 0, wa = 0;
+  bool late = false;  // wa's run starts before the sequence
+  if (p.own.n_waves > 0) {
+    const stream::BatchScan sc = stream::batch_scan<kPG, SK>(p.own, J);
+    const int L = sc.per == 1 ? __builtin_amdgcn_readlane(sc.L, b) : stream::seq_len<kPG>(p.own, b);
+    const int nst = (L + SK - 1) / SK;
+    if (nst > 0) {
+      const stream::Partition part(sc.tot, p.own.n_waves);
+      const int64_t s0 = stream::stages_before<kPG, SK>(p.own, J, b, sc) + (seq - (int64_t)b * J) * nst;
+      wa = part.wave_of(s0);
+      np = part.wave_of(s0 + nst - 1) - wa + 1;
+      late = part.start(wa) < s0;
     }
   }
-  __syncthreads();
-  const int np = found[0], wa = found[1];
-  const bool late = found[2] != 0;
-  const int npre = (prefix_len(p) + p.chunk - 1) / p.chunk;
-  const int total = npre + np;
+  join();
+  for (int s = NB * ngrp; s < npre; s += NB * ngrp) {
+    fetch(s, npre, p.part_o, p.part_ml, chunk_row);
+    join();
+  }
+  for (int s = 0; s < np; s += NB * ngrp) {
+    fetch(s, np, p.own.part_o, p.own.part_ml, [&](int k) {
+      return own_slot(p.own, J, wa + k, seq, np == 1, k == 0 && late) * p.own_rows + h0 - kRows * slice + qi;
+    });
+    join();
+  }
 
-  __shared__ f32x4 so[256];
-  __shared__ f32x2 sm[256];
-  const int per = nq * LPR;
-  const int ngrp = per >= 256 ? 1 : 256 / per;
-  const int grp = per >= 256 ? 0 : tid / per;
-  for (int i0 = 0; i0 < per; i0 += 256) {  // one round where per <= 256
-    const int i = per >= 256 ? i0 + tid : tid - grp * per;
-    const bool on = i < per && grp < ngrp;
-    const int qi = on ? i / LPR : 0, d0 = on ? 4 * (i % LPR) : 0;
-    const int64_t bh = (int64_t)b * p.Hq + kvh * g + h0 + qi;
-    float M = kNegInf, l = 0.f;
-    f32x4 o = (f32x4)(0.f);
-    for (int c0 = grp; on && c0 < total; c0 += NB * ngrp) {
-      f32x2 ml[NB];
-      f32x4 v[NB];
-      float Mn = M;
-#pragma unroll
-      for (int c = 0; c < NB; ++c) {
-        const int s = c0 + c * ngrp;
-        ml[c] = (f32x2){kNegInf, 0.f};
-        v[c] = (f32x4)(0.f);
-        if (s < total) {
-          const float *po = p.part_o, *pm = p.part_ml;
-          int64_t row = (int64_t)s * p.own.B * p.Hq + bh;
-          if (s >= npre) {
-            const int i1 = s - npre;
-            po = p.own.part_o;
-            pm = p.own.part_ml;
-            row = own_slot(p.own, J, wa + i1, seq, np == 1, i1 == 0 && late) * p.own_rows + h0 - kRows * slice + qi;
-          }
-          ml[c] = *reinterpret_cast<const f32x2*>(pm + row * 2);
-          v[c] = *reinterpret_cast<const f32x4*>(po + row * D + d0);
-        }
-        Mn = fmaxf(Mn, ml[c][0]);
-      }
-      const float Mu = (Mn == kNegInf) ? 0.f : Mn;
-      const float back = exp2f(M - Mu);
-      o *= back;
-      l *= back;
-#pragma unroll
-      for (int c = 0; c < NB; ++c) {
-        const float wt = exp2f(ml[c][0] - Mu);
-        l += ml[c][1] * wt;
-        o += v[c] * wt;
-      }
-      M = Mn;
+  if (ngrp > 1) {
+    __shared__ f32x4 so[256];
+    __shared__ f32x2 sm[256];
+    so[tid] = o;
+    sm[tid] = (f32x2){M, l};
+    __syncthreads();
+    if (grp != 0) return;
+    for (int k = 1; k < ngrp; ++k) M = fmaxf(M, sm[tid + k * per][0]);
+    const float Mu = (M == kNegInf) ? 0.f : M;
+    const float mine = exp2f(sm[tid][0] - Mu);
+    o *= mine;
+    l *= mine;
+    for (int k = 1; k < ngrp; ++k) {
+      const f32x2 x = sm[tid + k * per];
+      const float wt = exp2f(x[0] - Mu);
+      l += x[1] * wt;
+      o += so[tid + k * per] * wt;
     }
-    if (ngrp > 1) {
-      so[tid] = o;
-      sm[tid] = (f32x2){M, l};
-      __syncthreads();
-      if (grp != 0) return;
-      for (int k = 1; k < ngrp; ++k) M = fmaxf(M, sm[tid + k * per][0]);
-      const float Mu = (M == kNegInf) ? 0.f : M;
-      const float mine = exp2f(sm[tid][0] - Mu);
-      o *= mine;
-      l *= mine;
-      for (int k = 1; k < ngrp; ++k) {
-        const f32x2 x = sm[tid + k * per];
-        const float wt = exp2f(x[0] - Mu);
-        l += x[1] * wt;
-        o += so[tid + k * per] * wt;
-      }
-    }
-    if (on && d0 < p.dr) {
-      const float inv = (l == 0.f) ? 0.f : 1.f / l;  // no key, or none that weighs: o = 0
-      typedef T v4 __attribute__((ext_vector_type(4)));
-      v4 y;
+  }
+  if (on && d0 < p.dr) {
+    const float inv = (l == 0.f) ? 0.f : 1.f / l;  // no key, or none that weighs: o = 0
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    v4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f32(o[e] * inv);
-      *reinterpret_cast<v4*>(static_cast<T*>(p.o) + bh * p.dr + d0) = y;
-    }
+    for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f32(o[e] * inv);
+    *reinterpret_cast<v4*>(static_cast<T*>(p.o) + bh * p.dr + d0) = y;
   }
 }
 
@@ -935,17 +933,16 @@ hipError_t launch(const PrefixParams& p, hipStream_t st) {
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D, (PG > 0 ? kOwnKeys : kBN)>),
-                     dim3((unsigned)(p.own.B * p.Hkv * ((p.g + 15) / 16))), dim3(256), 0, st, p);
+                     dim3((unsigned)(p.own.B * p.Hkv * ((p.g + p.merge_heads - 1) / p.merge_heads))), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
 template <typename T, int D>
 hipError_t launch_pages(const PrefixParams& p, hipStream_t st) {
   if (!p.dma) return launch<T, D, 0, 0>(p, st);
-  if (!p.thin) return launch<T, D, 1, 0>(p, st);
   constexpr int PG = OwnGeo<T, D>::RPL == 8 ? 8 : 4;
-  if (p.page_size % 64 == 0) return launch<T, D, 64, 16>(p, st);
-  return p.page_size % 16 == 0 ? launch<T, D, 1, 16>(p, st) : launch<T, D, 1, PG>(p, st);
+  if (p.page_size % 16 == 0) return p.thin ? launch<T, D, 16, 16>(p, st) : launch<T, D, 16, 0>(p, st);
+  return p.thin ? launch<T, D, 1, PG>(p, st) : launch<T, D, 1, 0>(p, st);
 }
 
 template <typename T>

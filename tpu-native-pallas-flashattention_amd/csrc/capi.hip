@@ -879,18 +879,21 @@ int own_waves(const pf::PrefixParams& p, bool thin) {
   return (int)std::min(most, (int64_t)p.own.B * p.Hkv * p.n_hc * (((int64_t)p.own.pages_per_seq * p.page_size + keys - 1) / keys));
 }
 
-// The work: prefix chunks of at least 128 keys for an item per CU; the own keys
+// The work: prefix chunks of at least 64 keys for an item per CU; the own keys
 // over at most one workgroup per CU (two: 39 us for 34, 64
 // sequences over 2000 prefix keys), a wave (thin) or workgroup for as little as
 // one stage (by the longest lengths).
-void plan_prefix(pf::PrefixParams* p) {
+void plan_prefix(pf::PrefixParams* p, int D) {
   const int64_t items = (int64_t)p->n_tiles * p->Hkv;
   if (p->len > 0) {
     const int64_t n = std::max<int64_t>(1, kCus / items);
-    p->chunk = (int)std::max<int64_t>(128, ((p->len + n - 1) / n + 63) / 64 * 64);
+    p->chunk = (int)std::max<int64_t>(64, ((p->len + n - 1) / n + 63) / 64 * 64);
     p->n_split = (p->len + p->chunk - 1) / p->chunk;
   }
   p->own.n_waves = own_waves(*p, p->thin);
+  p->merge_heads = std::min(p->g, 1024 / D);
+  while (p->merge_heads > 1 && p->n_split > (int64_t)pf::kMergeLoads * (1024 / D / p->merge_heads))
+    p->merge_heads = (p->merge_heads + 1) / 2;
 }
 
 // *D: the compute head dim.
@@ -943,7 +946,7 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   // own_stream: at most 8 heads, whole rows of a kernel's head dim, whole page groups
   p->thin = p->dma && p->g <= 8 && a->head_dim == *D && a->page_size % std::max(4, rows_per_load) == 0 &&
             ((uintptr_t)a->q & 15) == 0;
-  if (a->batch > 0) plan_prefix(p);
+  if (a->batch > 0) plan_prefix(p, *D);
   const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
   if (n_pre + p->own.n_waves > kMaxGrid) return PF_ERR_UNSUPPORTED;
   p->n_pre = (int)n_pre;

@@ -338,6 +338,7 @@ hipError_t launch_decode_stream(const DecodeParams& p, int dtype, bool paged, hi
 
 // Attention of a batch over a shared prefix (attn_prefix.hip).
 constexpr int kPrefixRows = 128;  // query rows per workgroup
+constexpr int kMergeLoads = 8;    // partials in flight per lane of the merge
 struct PrefixParams {
   const void* q;  // [B, Hq, dr]
   const void* k;  // page pools
@@ -366,6 +367,7 @@ struct PrefixParams {
   int thin;
   int n_hc;      // ceil(g / kPrefixRows) slices of a KV head's query heads
   int own_rows;  // min(g, kPrefixRows)
+  int merge_heads;  // heads of a KV head per workgroup of the merge, at most 1024 / D; slices are whole multiples
 };
 hipError_t launch_prefix_f32(const PrefixParams& p, int D, hipStream_t stream);
 hipError_t launch_prefix_bf16(const PrefixParams& p, int D, hipStream_t stream);
