@@ -875,21 +875,49 @@ int pf_paged_attn(const pf_paged_attn_args* a, void* stream) {
 namespace {
 
 int own_waves(const pf::PrefixParams& p, bool thin) {
-  const int64_t keys = thin ? 16 : 64, most = thin ? 4 * kCus : kCus;
+  const int64_t keys = thin ? 16 : 64, most = (thin ? 4 : 1) * (int64_t)p.own_cus;
   return (int)std::min(most, (int64_t)p.own.B * p.Hkv * p.n_hc * (((int64_t)p.own.pages_per_seq * p.page_size + keys - 1) / keys));
 }
 
-// The work: prefix chunks of at least 64 keys for an item per CU; the own keys
-// over at most one workgroup per CU (two: 39 us for 34, 64
-// sequences over 2000 prefix keys), a wave (thin) or workgroup for as little as
-// one stage (by the longest lengths).
-void plan_prefix(pf::PrefixParams* p, int D) {
+// The work: the prefix in n_tiles Hkv n_split items of at least 64 keys; the own
+// keys over own_cus workgroups, a wave (thin) or workgroup for as little as one
+// stage (by the longest lengths).
+//
+// Two or more workgroups per CU (rows under 512 bytes): an item per CU and own
+// keys over another workgroup per CU. Items of many rows and few keys move more in
+// partials (written and read, 8 rows D bytes) than in keys (2 chunk row bytes):
+// then items for half the CUs, up to three keys a row (bfloat16, head_dim 128: 31
+// chunks of 192 keys 34.5 us, 16 of 384 31.4, 128 rows beside long own keys; 4 of
+// 256 52 us, 8 of 128 59, 512 rows; but 32 rows, 2000 keys: 64 keys 14.5, 128 16).
+//
+// One workgroup per CU: both kinds at once on the CUs, in proportion to their work
+// (own keys: half the bound; a prefix key of 128 rows costs an own key's time in
+// 16 bits, three times that in float32), the prefix on half at least, as the bound
+// may be far off. (float16, head_dim 256, 16 sequences over 5003 keys: one after
+// the other 30.6 us, half and half 26; 128 over 16384: 205, 171; 16 over 40000,
+// nearly all of it the prefix's: 70, 88.)
+void plan_prefix(pf::PrefixParams* p, int D, int es) {
   const int64_t items = (int64_t)p->n_tiles * p->Hkv;
+  const bool one = D * es >= 512;
+  int64_t cus = kCus;  // the prefix's
+  if (one) {
+    const double pre = (double)p->n_tiles * p->len * (es == 4 ? 3 : 1);
+    const double own = 0.5 * p->own.B * p->n_hc * (double)p->own.pages_per_seq * p->page_size;
+    if (own > 0) cus = std::min<int64_t>(kCus - 8, std::max<int64_t>(kCus / 2, (int64_t)(kCus * (pre / (pre + own)))));
+  }
   if (p->len > 0) {
-    const int64_t n = std::max<int64_t>(1, kCus / items);
-    p->chunk = (int)std::max<int64_t>(64, ((p->len + n - 1) / n + 63) / 64 * 64);
+    const auto keys = [&](int64_t c) {  // per chunk, for an item on each of c CUs
+      const int64_t n = std::max<int64_t>(1, c / items);
+      return ((p->len + n - 1) / n + 63) / 64 * 64;
+    };
+    p->chunk = (int)std::max<int64_t>(64, keys(cus));
+    if (!one) {
+      const int64_t rows3 = 3 * std::min(p->rows, pf::kPrefixRows) / 64 * 64;
+      p->chunk = (int)std::max<int64_t>(p->chunk, std::min(keys(kCus / 2), rows3));
+    }
     p->n_split = (p->len + p->chunk - 1) / p->chunk;
   }
+  p->own_cus = one ? (int)std::max<int64_t>(kCus - cus, kCus - items * p->n_split) : kCus;
   p->own.n_waves = own_waves(*p, p->thin);
   p->merge_heads = std::min(p->g, 1024 / D);
   while (p->merge_heads > 1 && p->n_split > (int64_t)pf::kMergeLoads * (1024 / D / p->merge_heads))
@@ -946,7 +974,7 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   // own_stream: at most 8 heads, whole rows of a kernel's head dim, whole page groups
   p->thin = p->dma && p->g <= 8 && a->head_dim == *D && a->page_size % std::max(4, rows_per_load) == 0 &&
             ((uintptr_t)a->q & 15) == 0;
-  if (a->batch > 0) plan_prefix(p, *D);
+  if (a->batch > 0) plan_prefix(p, *D, a->dtype == PF_DTYPE_F32 ? 4 : 2);
   const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
   if (n_pre + p->own.n_waves > kMaxGrid) return PF_ERR_UNSUPPORTED;
   p->n_pre = (int)n_pre;

@@ -365,6 +365,7 @@ struct PrefixParams {
   // waves (own_stream); else in blocks of 64 keys over n_waves workgroups.
   DecodeParams own;
   int thin;
+  int own_cus;   // workgroups of own keys, at most
   int n_hc;      // ceil(g / kPrefixRows) slices of a KV head's query heads
   int own_rows;  // min(g, kPrefixRows)
   int merge_heads;  // heads of a KV head per workgroup of the merge, at most 1024 / D; slices are whole multiples
