@@ -58,6 +58,7 @@ constexpr int kRows = kPrefixRows;
 
 constexpr int kPG = 2;  // the work list's lengths are those of a paged call
 using stream::Cursor;
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 __device__ inline int prefix_len(const PrefixParams& p) {
   return p.len_ptr != nullptr ? min(max(stream::sload_i32(p.len_ptr, 0), 0), p.len) : p.len;
@@ -70,6 +71,16 @@ __device__ inline int prefix_len(const PrefixParams& p) {
 __device__ inline int64_t own_slot(const DecodeParams& p, int J, int w, int64_t seq, bool whole, bool late) {
   if (whole && (int64_t)p.B * J > p.n_waves) return 2 * (int64_t)p.n_waves + seq;
   return stream::piece_slot(p, J, w, seq, late);
+}
+
+// What the merge has to know of a sequence's own pieces, left by the workgroup or
+// wave w whose piece opens it (c: that piece's last stage): w, whether the piece is
+// not w's first, and how many pieces there are, w's and its successors'.
+__device__ inline void own_note(const PrefixParams& p, const stream::Partition& part, int w, int64_t seq,
+                                const Cursor& c, bool late) {
+  int np = 1;
+  if (c.st < c.nst - 1) np += part.wave_of(part.start(w + 1) + (c.nst - 2 - c.st)) - w;
+  reinterpret_cast<i32x2*>(p.own_info)[seq] = (i32x2){2 * w + (late ? 1 : 0), np};
 }
 
 // Loads of 64-row tiles: the keys [64 st, ...) below L of the cursor's sequence.
@@ -389,7 +400,9 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
       l_tot = wave_xor32_sum(l_tot);
       if (i16 < g) {
         const bool whole = piece_st0 == 0 && cc.st == cc.nst - 1;
-        const int64_t at = own_slot(own, J, w, (int64_t)cc.b * J + cc.j, whole, !first_piece) * g + i16;
+        const int64_t seq = (int64_t)cc.b * J + cc.j;
+        if (piece_st0 == 0 && lane == 0) own_note(p, part, w, seq, cc, !first_piece);
+        const int64_t at = own_slot(own, J, w, seq, whole, !first_piece) * g + i16;
         float* po = own.part_o + at * D;
 #pragma unroll
         for (int q = 0; q < NACC; ++q) {
@@ -428,6 +441,7 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   // The workgroup's n blocks and the first one's cursor.
   Cursor cp;
   int n, r0 = 0, piece = 0;
+  [[maybe_unused]] stream::Partition part((int64_t)0, (int64_t)0);
   if constexpr (!OWN) {
     // (chunk, kv head, row tile): the row tiles of one chunk side by side on one
     // XCD, whose L2 then serves the chunk to all of them.
@@ -438,7 +452,6 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
     n = (L - key0 + kBN - 1) / kBN;
     cp = Cursor{0, it / p.n_tiles % p.Hkv, key0 / kBN, key0 / kBN + n, L};
   } else {
-    stream::Partition part((int64_t)0, (int64_t)0);
     n = (int)stream::wave_plan<kPG, kBN>(p.own, J, p.own.n_waves, item, &cp, &part);
   }
   n = __builtin_amdgcn_readfirstlane(n);  // barriers are counted by it
@@ -643,6 +656,7 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
       if constexpr (OWN) {
         const int64_t seq = (int64_t)c.b * J + c.j;
         const bool whole_seq = piece_st0 == 0 && c.st == c.nst - 1;
+        if (piece_st0 == 0 && w32 == 0 && lane == 0) own_note(p, part, item, seq, c, !first_piece);
         at = own_slot(p.own, J, item, seq, whole_seq, !first_piece) * p.own_rows + w32 + l32;
         po = p.own.part_o;
         pm = p.own.part_ml;
@@ -811,11 +825,11 @@ void pf_prefix_kernel(PrefixParams p) {
 // lanes a row, 16 bytes each; groups of lanes share the chunks and pieces and join
 // through LDS. The kv head is the innermost index, as that of the prefix items: an
 // XCD mostly reads what its own L2 still holds (31 chunks of 192 keys, 32 sequences,
-// both launches: 29 -> 21 us). Bound by latency: the chunks' partials, 8 in flight per lane, are on
-// their way while each wave finds the sequence's pieces in the work list.
+// both launches: 29 -> 21 us). Bound by latency: the chunks' partials, 8 in flight
+// per lane, are on their way while the note of the own pieces comes.
 // merge_heads is such that the chunks are one round of loads, where it can be.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int SK>
+template <typename T, int D>
 __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
   constexpr int LPR = D / 4, NB = kMergeLoads;
   const int g = p.g, nh = p.merge_heads, n_h = (g + nh - 1) / nh;
@@ -867,23 +881,16 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
   auto chunk_row = [&](int s) { return (int64_t)s * p.own.B * p.Hq + bh; };
   fetch(0, npre, p.part_o, p.part_ml, chunk_row);
 
-  // The sequence's np pieces: of wa and the workgroups (waves) after it.
+  // The sequence's pieces, if it has keys (else nothing was noted).
   const int J = p.Hkv * p.n_hc, slice = h0 / kRows;
   const int64_t seq = (int64_t)b * J + kvh * p.n_hc + slice;
-  int np = 0, wa = 0;
-  bool late = false;  // wa's run starts before the sequence
+  i32x2 note = (i32x2){0, 0};
   if (p.own.n_waves > 0) {
-    const stream::BatchScan sc = stream::batch_scan<kPG, SK>(p.own, J);
-    const int L = sc.per == 1 ? __builtin_amdgcn_readlane(sc.L, b) : stream::seq_len<kPG>(p.own, b);
-    const int nst = (L + SK - 1) / SK;
-    if (nst > 0) {
-      const stream::Partition part(sc.tot, p.own.n_waves);
-      const int64_t s0 = stream::stages_before<kPG, SK>(p.own, J, b, sc) + (seq - (int64_t)b * J) * nst;
-      wa = part.wave_of(s0);
-      np = part.wave_of(s0 + nst - 1) - wa + 1;
-      late = part.start(wa) < s0;
-    }
+    note = reinterpret_cast<const i32x2*>(p.own_info)[seq];
+    if (stream::seq_len<kPG>(p.own, b) <= 0) note = (i32x2){0, 0};
   }
+  const int wa = note[0] >> 1, np = note[1];
+  const bool late = (note[0] & 1) != 0;
   join();
   for (int s = NB * ngrp; s < npre; s += NB * ngrp) {
     fetch(s, npre, p.part_o, p.part_ml, chunk_row);
@@ -934,7 +941,7 @@ hipError_t launch(const PrefixParams& p, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D, (PG > 0 ? kOwnKeys : kBN)>),
+  hipLaunchKernelGGL((pf_prefix_merge_kernel<T, D>),
                      dim3((unsigned)(p.own.B * p.Hkv * ((p.g + p.merge_heads - 1) / p.merge_heads))), dim3(256), 0, st, p);
   return hipGetLastError();
 }

@@ -993,7 +993,8 @@ size_t own_piece_rows(const pf::PrefixParams& p) {
   return std::max(form_piece_rows(p, true), form_piece_rows(p, false));
 }
 size_t prefix_ws(const pf::PrefixParams& p, int D) {
-  return std::max<size_t>(partial_bytes(prefix_rows(p), D) + partial_bytes(own_piece_rows(p), D), 256);
+  const size_t notes = align256((size_t)p.own.B * p.Hkv * p.n_hc * 8);
+  return std::max<size_t>(partial_bytes(prefix_rows(p), D) + partial_bytes(own_piece_rows(p), D) + notes, 256);
 }
 
 }  // namespace
@@ -1020,6 +1021,7 @@ int pf_paged_prefix_attn(const pf_paged_prefix_attn_args* a, void* stream) {
   ws += partial_bytes(prefix_rows(p), D);
   p.own.part_o = reinterpret_cast<float*>(ws);
   p.own.part_ml = reinterpret_cast<float*>(ws + align256(own_piece_rows(p) * D * sizeof(float)));
+  p.own_info = reinterpret_cast<int32_t*>(ws + partial_bytes(own_piece_rows(p), D));
   return finish(pf::launch_prefix(p, a->dtype, D, (hipStream_t)stream));
 }
 

@@ -364,6 +364,7 @@ struct PrefixParams {
   // partials, own_rows rows per slot. thin: in stages of 16 keys over n_waves
   // waves (own_stream); else in blocks of 64 keys over n_waves workgroups.
   DecodeParams own;
+  int32_t* own_info;  // [B Hkv n_hc, 2]: where each sequence's pieces are
   int thin;
   int own_cus;   // workgroups of own keys, at most
   int n_hc;      // ceil(g / kPrefixRows) slices of a KV head's query heads
