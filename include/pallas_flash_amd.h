@@ -438,6 +438,8 @@ int pf_paged_cache_write(const pf_paged_cache_write_args* args, void* stream);
  *   cos, sin [rope_len, head_dim] float32
  *   axes in [1, 4]; sections positive, head_dim / 2 in all
  *   head_dim: even, any
+ * More than 65535 heads (q and k together), or batch * head_dim near 2^32:
+ * PF_ERR_UNSUPPORTED.
  * ------------------------------------------------------------------------- */
 #define PF_MAX_ROPE_AXES 4
 typedef struct {

@@ -158,6 +158,19 @@ def test_work_lists(dt, batch, hq, hkv, d, page, prefix, hi):
     check(make(dt, batch, hq, hkv, d, page, prefix, lens, poison=False), dt)
 
 
+@pytest.mark.parametrize("dt,batch,hq,hkv,d,page,prefix,lens", [
+    ("bf16", 1, 4, 1, 128, 16, 0, [30000]),        # one sequence over every wave
+    ("f16", 1, 20, 1, 64, 16, 77, [30000]),        # ... over every workgroup
+    ("f32", 2, 16, 1, 128, 16, 9000, [5000, 3]),   # one workgroup per CU
+    ("f16", 2, 16, 1, 256, 16, 9000, [40, 900]),
+    ("bf16", 48, 64, 2, 128, 64, 1300, [5] * 48),  # 12 tiles of rows, few keys
+    ("bf16", 300, 16, 16, 64, 64, 3, [0] * 300),   # more items than CUs, nothing of one's own
+])
+def test_splits(dt, batch, hq, hkv, d, page, prefix, lens):
+    note(f"prefix {dt} B={batch} {hq}/{hkv} D={d} page={page} prefix={prefix} lens={lens[:4]}")
+    check(make(dt, batch, hq, hkv, d, page, prefix, lens, poison=False), dt)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("waves,stages", [(1, 2), (7, 3), (64, 4)])
 def test_tuned_grids(dt, waves, stages):

@@ -125,3 +125,10 @@ def test_c_dtypes_empty_and_null(L):
     for empty in (dict(batch=0), dict(seq_len=0)):
         assert L.pf_rope_axes(axes_args(**empty), None) == _lib.PF_OK
         assert L.pf_rope_paged_cache_write(write_args(**empty), None) == _lib.PF_OK
+
+
+@pytest.mark.parametrize("over", [dict(num_heads=65536), dict(num_heads=65532, num_kv_heads=4),
+                                  dict(batch=1 << 26, seq_len=1)])
+def test_c_sizes_past_the_grid_refused(L, over):
+    assert L.pf_rope_axes(axes_args(**over), None) == _lib.PF_ERR_UNSUPPORTED
+    assert L.pf_rope_paged_cache_write(write_args(**over), None) == _lib.PF_ERR_UNSUPPORTED

@@ -1168,6 +1168,11 @@ static int fill_rope_axes(int32_t axes, const int32_t* sections, const float* co
   return PF_OK;
 }
 
+// What the launch counts in 32 bits and the grid's second axis.
+static bool rope_grid_ok(const pf::RopeAxesParams& p, int64_t heads) {
+  return heads <= 65535 && (int64_t)p.B * p.D <= ((int64_t)1 << 32) - 1024;
+}
+
 static void set_rope_input(pf::RopeAxesParams* p, int i, const void* x, const int64_t* stride, int heads, void* out) {
   p->x[i] = x;
   p->sb[i] = stride[0];
@@ -1191,6 +1196,7 @@ int pf_rope_axes(const pf_rope_axes_args* a, void* stream) {
   p.positions = a->positions;
   for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->positions_stride[i];
   p.inverse = a->inverse;
+  if (!rope_grid_ok(p, (int64_t)a->num_heads + a->num_kv_heads)) return PF_ERR_UNSUPPORTED;
   return finish(pf::launch_rope_axes(p, a->dtype, false, (hipStream_t)stream));
 }
 
@@ -1220,6 +1226,7 @@ int pf_rope_paged_cache_write(const pf_rope_paged_write_args* a, void* stream) {
   p.num_pages = a->num_pages;
   p.page_size = a->page_size;
   p.pages_per_seq = a->pages_per_seq;
+  if (!rope_grid_ok(p, (int64_t)a->num_heads + 2 * (int64_t)a->num_kv_heads)) return PF_ERR_UNSUPPORTED;
   return finish(pf::launch_rope_axes(p, a->dtype, true, (hipStream_t)stream));
 }
 

@@ -250,7 +250,6 @@ hipError_t launch_heads(RopeAxesParams p, hipStream_t st) {
   p.div_page = fast_divisor(APPEND ? p.page_size : 1);
   // 32-bit items: past 2^31 of them, the tokens in several launches.
   const int64_t most = (((int64_t)1 << 31) - 256) / ((int64_t)p.B * chunks);
-  if (most < 1 || groups > 65535) return hipErrorInvalidValue;
   const int seq = p.S;
   for (int s0 = 0; s0 < seq; s0 += (int)std::min<int64_t>(most, seq)) {
     const int n = (int)std::min<int64_t>(most, seq - s0);
