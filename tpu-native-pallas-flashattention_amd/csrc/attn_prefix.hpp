@@ -120,23 +120,35 @@ struct PageTiles {
     }
   }
   __device__ inline int kv_head(const Cursor& c) const { return n_hc == 1 ? c.j : c.j / n_hc; }
-  // The byte offsets in the pool where a block's lookups start (wave-uniform;
-  // scalar loads of the table, which do not disturb the count of the loads in
-  // flight), and the bytes behind them that are valid. A lookup past the table's
-  // reach takes the last page and reads nothing.
+  // The pages of a block's lookups (wave-uniform: scalar loads of the table, which
+  // do not disturb the count of the loads in flight), asked for a block before
+  // rows() takes them. A lookup past the table's reach takes the last page and
+  // reads nothing.
+  struct Pages {
+    int id[NG];
+  };
+  __device__ inline int key_of(const Cursor& c, int u) const {
+    return kBN * c.st + row0 + GR * u;
+  }
+  __device__ inline int logical(int key) const { return min((int)fast_div(key, p.div_page), pages - 1); }
+  __device__ inline Pages look(const Cursor& c) const {
+    Pages x;
+#pragma unroll
+    for (int u = 0; u < NG; ++u) x.id[u] = stream::sload_i32(table, (int64_t)c.b * pages + logical(key_of(c, u)));
+    return x;
+  }
+  // The byte offsets in the pool where they start, and the valid bytes behind them.
   struct Rows {
     uint64_t at[NG];
     uint32_t bytes[NG];
   };
-  __device__ inline Rows rows(const Cursor& c) const {
+  __device__ inline Rows rows(const Cursor& c, const Pages& page) const {
     Rows x;
     const int kvh = kv_head(c);
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
-      const int key = kBN * c.st + row0 + GR * u;
-      const int lp = min((int)fast_div(key, p.div_page), pages - 1);
-      const int page = min(max(stream::sload_i32(table, (int64_t)c.b * pages + lp), 0), p.num_pages - 1);
-      x.at[u] = (uint64_t)(((uint32_t)page * p.Hkv + kvh) * p.page_size + (key - lp * p.page_size)) * rb;
+      const int key = key_of(c, u), id = min(max(page.id[u], 0), p.num_pages - 1);
+      x.at[u] = (uint64_t)(((uint32_t)id * p.Hkv + kvh) * p.page_size + (key - logical(key) * p.page_size)) * rb;
       x.bytes[u] = min(max(c.L - key, 0), GR) * rb;
     }
     return x;
@@ -484,12 +496,13 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
     }
   };
 
-  // Cursors of blocks t (cp) .. t + 3 (cl), and where the loads of blocks t + 1 ..
-  // t + 3 start.
+  // Cursors of blocks t (cp) .. t + 4 (cm), where the loads of blocks t + 1 .. t + 3
+  // start, and the pages of block t + 4.
   char* const kbuf = smem;  // K tiles t & 1, then V tiles
   char* const vbuf = smem + 2 * G::BYTES;
-  Cursor cs = after(cp, 0), ck = after(cs, 1), cl = after(ck, 2);
+  Cursor cs = after(cp, 0), ck = after(cs, 1), cl = after(ck, 2), cm = after(cl, 3);
   typename PTiles::Rows r1, r2, r3;
+  typename PTiles::Pages next;
   auto whole = [&](const void* pool, [[maybe_unused]] const Cursor& c, const typename PTiles::Rows& x, char* tile) {
     if constexpr (DMA == 16) {
       const i32x4 d = tiles.rows_desc(pool, x);
@@ -505,10 +518,12 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   {
     typename PTiles::Rows r;
     if constexpr (DMA > 0) {
-      r = tiles.rows(cp);
-      r1 = tiles.rows(cs);
-      r2 = tiles.rows(ck);
-      r3 = tiles.rows(cl);
+      const auto p0 = tiles.look(cp), p1 = tiles.look(cs), p2 = tiles.look(ck), p3 = tiles.look(cl);
+      next = tiles.look(cm);
+      r = tiles.rows(cp, p0);
+      r1 = tiles.rows(cs, p1);
+      r2 = tiles.rows(ck, p2);
+      r3 = tiles.rows(cl, p3);
     }
     whole(p.k, cp, r, kbuf);
     whole(p.k, cs, r1, kbuf + G::BYTES);
@@ -546,11 +561,13 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
     cp = cs;
     cs = ck;
     ck = cl;
-    cl = after(cl, t + 3);
+    cl = cm;
+    cm = after(cm, t + 4);
     if constexpr (DMA > 0) {
       r1 = r2;
       r2 = r3;
-      r3 = tiles.rows(cl);
+      r3 = tiles.rows(cl, next);
+      next = tiles.look(cm);
     }
     wait_vm<2 * PT>();  // K_{t+2}: V_{t+1} and K_{t+3} were asked for after it
     __syncthreads();

@@ -889,27 +889,34 @@ int own_waves(const pf::PrefixParams& p, bool thin) {
 // then items for half the CUs, up to three keys a row (bfloat16, head_dim 128: 31
 // chunks of 192 keys 34.5 us, 16 of 384 31.4, 128 rows beside long own keys; 4 of
 // 256 52 us, 8 of 128 59, 512 rows; but 32 rows, 2000 keys: 64 keys 14.5, 128 16).
+// Where the prefix is nearly all the work and its chunks stay long, two items per
+// CU (bfloat16, head_dim 128, 512 rows over 32768 keys, own keys to 64: 90 us, one
+// item 94; head_dim 64, 16384: 37, 40; but own keys to 500: 109, 101, and chunks of
+// 128 keys: 44, 36).
 //
-// One workgroup per CU: both kinds at once on the CUs, in proportion to their work
-// (own keys: half the bound; a prefix key of 128 rows costs an own key's time in
-// 16 bits, three times that in float32), the prefix on half at least, as the bound
-// may be far off. (float16, head_dim 256, 16 sequences over 5003 keys: one after
-// the other 30.6 us, half and half 26; 128 over 16384: 205, 171; 16 over 40000,
-// nearly all of it the prefix's: 70, 88.)
+// One workgroup per CU: both kinds at once on the CUs, in proportion to their
+// work, the prefix on half at least, as the own keys' bound may be far off.
+// (float16, head_dim 256, 16 sequences over 5003 keys: one after the other 30.6 us,
+// half and half 26; 128 over 16384: 205, 174; 16 over 40000, nearly all of it the
+// prefix's: 70, 88, in proportion 67.)
 void plan_prefix(pf::PrefixParams* p, int D, int es) {
   const int64_t items = (int64_t)p->n_tiles * p->Hkv;
   const bool one = D * es >= 512;
+  const auto keys = [&](int64_t c) {  // per chunk, for an item on each of c CUs
+    const int64_t n = std::max<int64_t>(1, c / items);
+    return ((p->len + n - 1) / n + 63) / 64 * 64;
+  };
+  // Work per KV head. A prefix key of up to 128 rows costs an own key's time in 16
+  // bits, three times that in float32; own keys: half their bound.
+  const double pre = (double)p->n_tiles * p->len * (es == 4 ? 3 : 1);
+  const double own = 0.5 * p->own.B * p->n_hc * (double)p->own.pages_per_seq * p->page_size;
   int64_t cus = kCus;  // the prefix's
   if (one) {
-    const double pre = (double)p->n_tiles * p->len * (es == 4 ? 3 : 1);
-    const double own = 0.5 * p->own.B * p->n_hc * (double)p->own.pages_per_seq * p->page_size;
     if (own > 0) cus = std::min<int64_t>(kCus - 8, std::max<int64_t>(kCus / 2, (int64_t)(kCus * (pre / (pre + own)))));
+  } else if (pre > 4 * own && keys(2 * kCus) >= 1024) {
+    cus = 2 * kCus;
   }
   if (p->len > 0) {
-    const auto keys = [&](int64_t c) {  // per chunk, for an item on each of c CUs
-      const int64_t n = std::max<int64_t>(1, c / items);
-      return ((p->len + n - 1) / n + 63) / 64 * 64;
-    };
     p->chunk = (int)std::max<int64_t>(64, keys(cus));
     if (!one) {
       const int64_t rows3 = 3 * std::min(p->rows, pf::kPrefixRows) / 64 * 64;
