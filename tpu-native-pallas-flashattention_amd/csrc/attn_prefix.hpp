@@ -31,11 +31,13 @@
 // that such loads would straddle and unaligned pools are staged through registers
 // instead.
 // Measured (bfloat16, head_dim 128, 32 heads over 8, 128 sequences, 32768 prefix
-// keys): the prefix alone 98 us, 702 TFLOP/s. One wave a SIMD leaves the pipeline
-// bound by its instructions; what helped was one lookup and descriptor per tile
-// and wave, tile addresses that are constants of each block's copy, and
-// nothing of the own keys' code in the loop. With the own keys (4.3 MB a sequence)
-// 144 us: 98 us of reads beside 98 us of products that share the SIMDs.
+// keys): the prefix alone 94 us with an item per CU, 90 (764 TFLOP/s) with two. One
+// wave a SIMD leaves the pipeline bound by its instructions and their latencies;
+// what helped was one lookup and descriptor per tile and wave, tile addresses that
+// are constants of each block's copy, nothing of the own keys' code in the loop (177
+// us for prefix and own keys -> 144), and page lookups a block ahead (142 -> 136).
+// With the own keys (4.3 MB a sequence, 96 us alone, 5.6 TB/s) 136 us: reads beside
+// products that share the SIMDs. 32 sequences over 6000 keys: 31 us.
 //
 // Own keys with at most 8 heads a KV head: the workgroup's waves each stream a
 // run of their own (own_stream). More heads, stored head dims that are not a
