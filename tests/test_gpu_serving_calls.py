@@ -149,3 +149,16 @@ def test_declines_the_rest():
     for i, bad in other.items():
         for x in bad:
             assert c.prefix(*a[:i], x, *a[i + 1:]) is None, (i, x)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_sizes_past_the_grid(grad):
+    """Refused before any launch, by the extension and by the general path."""
+    q = r(1, 65536, 1, 2).requires_grad_(grad)
+    t = torch.ones(4, 2, device="cuda")
+    at = torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(NotImplementedError):
+        apply_rope_axes(q, None, at, t, t)
+    with general_path(), pytest.raises(NotImplementedError):
+        apply_rope_axes(q, None, at, t, t)
+    assert torch.equal(apply_rope_axes(q[:, :65535], None, at, t, 0 * t)[0], q[:, :65535])

@@ -527,6 +527,7 @@ std::vector<Tensor> rotate(const Tensor& q, const Tensor& k, pf_rope_axes_args a
   a.dtype = dtype_tag(q1);
   const int st = pf_rope_axes(&a, stream_of(q1));
   TORCH_CHECK_VALUE(st != PF_ERR_INVALID, "apply_rope_axes: invalid arguments (rejected by the C ABI)");
+  TORCH_CHECK_NOT_IMPLEMENTED(st != PF_ERR_UNSUPPORTED, "apply_rope_axes: unsupported sizes");
   TORCH_CHECK(st == PF_OK, "apply_rope_axes: HIP launch failed (status ", st, ")");
   return out;
 }
