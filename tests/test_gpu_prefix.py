@@ -246,6 +246,24 @@ def test_scores_without_weight(dt):
     assert (got[0].double() - want[0].double()).abs().max() <= 2 * torch.finfo(q.dtype).eps * want.abs().max() + 1e-6
 
 
+@pytest.mark.parametrize("page", [16, 12])
+def test_pools_past_32_bits(page):
+    """Pages behind 2^32 elements of a pool: the bits of a small pool's, for the append and the attention."""
+    q, k, v, ptab, prefix, table, lens = make("bf16", 3, 8, 2, 128, page, 200, [30, 0, 55], poison=False)
+    far = (1 << 32) // k[0].numel() + 3
+    kf, vf = (torch.empty(far + x.shape[0], *x.shape[1:], dtype=x.dtype, device="cuda") for x in (k, v))
+    kf[far:], vf[far:] = k, v
+    move = lambda t: torch.where(t < 0, t, t + far)  # noqa: E731
+    cos, sin = precompute_rope(100, 128, 10000.0, device="cuda")
+    x = torch.randn(3, 12, 4, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(q.dtype)
+    at = torch.tensor([30, 0, 55], device="cuda", dtype=torch.int32)
+    for kp, vp, tab in ((k, v, table), (kf, vf, move(table))):
+        write_to_paged_cache_rope(kp, vp, x[:, :8], x[:, 8:10], x[:, 10:], tab, at, cos, sin)
+    assert torch.equal(kf[far:], k) and torch.equal(vf[far:], v)
+    near = check((q, k, v, ptab, prefix, table, lens), "bf16")
+    assert torch.equal(near, paged_flash_attention_prefix(q, kf, vf, move(ptab), prefix, move(table), lens))
+
+
 def test_prefix_length_on_the_device_captured():
     """One captured call follows a prefix and contexts that grow; replays on a side stream, eager work between them."""
     q, k, v, ptab, _, table, lens = make("bf16", 6, 8, 2, 128, 16, 640, [30, 0, 500, 64, 10, 1], poison=False)

@@ -374,3 +374,26 @@ def test_large_calls(dt, hq, hk, d):
     assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
     keep = (pos >= 0).all(0)[:, None, :, None] & (torch.arange(s, device="cuda") < lens[:, None])[:, None, :, None]
     assert torch.equal(qa, torch.where(keep, qr, torch.zeros_like(qr))) and pools[0].any()
+
+
+def test_rotation_past_32_bits():
+    """Heads behind 2^32 bytes: the bits of the same heads alone, forward and backward, dense and strided."""
+    b, h, s, d = 2, 20, 220000, 256
+    cos, sin = tables(300, d)
+    pos = torch.randint(0, 300, (2, b, s), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    last = torch.randn(b, 1, s, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).half()
+    for dims in ((b, h, s, d), (b, s, h, d)):
+        x = torch.zeros(dims, dtype=torch.float16, device="cuda")
+        assert x.numel() > 1 << 31
+        x = x if dims[1] == h else x.transpose(1, 2)
+        x[:, -1:] = last
+        out, _ = apply_rope_axes(x, None, pos, cos, sin, (50, 78))
+        want, _ = apply_rope_axes(last, None, pos, cos, sin, (50, 78))
+        assert torch.equal(out[:, -1:], want) and not out[:, :-1].any()
+        y = last.clone().requires_grad_()
+        want, = torch.autograd.grad(apply_rope_axes(y, None, pos, cos, sin, (50, 78))[0], y, last)
+        del out
+        z = torch.zeros_like(x).requires_grad_()
+        got, = torch.autograd.grad(apply_rope_axes(z, None, pos, cos, sin, (50, 78))[0], z, x)
+        assert torch.equal(got[:, -1:], want)
+        del x, z, got
