@@ -40,8 +40,8 @@
 // products that share the SIMDs. 32 sequences over 6000 keys: 31 us.
 //
 // Own keys with at most 8 heads a KV head: the workgroup's waves each stream a
-// run of their own (own_stream). More heads, stored head dims that are not a
-// kernel's, odd pages and unaligned operands: the workgroup runs the prefix
+// run of their own (own_stream). More heads, odd pages and unaligned operands: the
+// workgroup runs the prefix
 // items' pipeline over its run, across the sequences: the block after a
 // sequence's last one is the next sequence's first.
 #pragma once
@@ -58,6 +58,7 @@ namespace prefix {
 constexpr int kBN = 64;      // keys per block
 constexpr int kRows = kPrefixRows;
 
+constexpr uint32_t kPastRange = 0x7ffffff0u;  // an offset past any load's buffer range
 constexpr int kPG = 2;  // the work list's lengths are those of a paged call
 using stream::Cursor;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
@@ -118,7 +119,7 @@ struct PageTiles {
       const int row = RPL * u + lane / G::CPR;
       const int chunk = (lane % G::CPR) ^ tile_swz<G::CPR>(16 * w + row);
       // columns past the stored row: past any range
-      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((row % GR * p.dr + chunk * G::EPC) * G::ES) : 0x7ffffff0u;
+      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((row % GR * p.dr + chunk * G::EPC) * G::ES) : kPastRange;
     }
   }
   __device__ inline int kv_head(const Cursor& c) const { return n_hc == 1 ? c.j : c.j / n_hc; }
@@ -247,11 +248,14 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   char* const qbuf = ring + 4 * G::TILE;   // sequences in turn
 
   // The chunk that this lane fetches for load i: its byte offset within the page group.
+  // (Columns past the stored row: past any range.)
+  const uint32_t rb = p.dr * sizeof(T);
   uint32_t loff[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int row = G::RPL * i + lane / G::CPR, c = lane % G::CPR;
-    loff[i] = (uint32_t)((row % PG) * RB + 16 * (c ^ G::swz(row)));
+    const int row = G::RPL * i + lane / G::CPR;
+    const uint32_t at = 16 * ((lane % G::CPR) ^ G::swz(row));
+    loff[i] = at < rb ? row % PG * rb + at : kPastRange;
   }
   // A stage's page groups: pool row and valid rows of each. Groups past the
   // length load nothing and look nothing up (-1 padding).
@@ -276,17 +280,18 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
     const uint32_t at = lds_u32(tile);
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      const i32x4 d = make_desc(static_cast<const char*>(pool) + (uint64_t)s.row[i] * RB, s.valid[i] * RB);
+      const i32x4 d = make_desc(static_cast<const char*>(pool) + (uint64_t)s.row[i] * rb, s.valid[i] * rb);
 #pragma unroll
       for (int e = 0; e < kPer; ++e) dma16<true>(d, loff[i * kPer + e], at + 1024 * (i * kPer + e));
     }
   };
   auto load_q = [&](const Cursor& c, char* q) {
-    const i32x4 d = make_desc(static_cast<const T*>(p.q) + ((int64_t)c.b * p.Hq + (int64_t)c.j * g) * D, g * RB);
+    const i32x4 d = make_desc(static_cast<const T*>(p.q) + ((int64_t)c.b * p.Hq + (int64_t)c.j * g) * p.dr, g * rb);
 #pragma unroll
     for (int i = 0; i < G::QB / 1024; ++i) {
-      const int row = G::RPL * i + lane / G::CPR, c16 = lane % G::CPR;
-      dma16(d, (uint32_t)(row * RB + 16 * (c16 ^ (row & G::QMASK))), lds_u32(q) + 1024 * i);
+      const int row = G::RPL * i + lane / G::CPR;
+      const uint32_t at = 16 * ((lane % G::CPR) ^ (row & G::QMASK));
+      dma16(d, at < rb ? row * rb + at : kPastRange, lds_u32(q) + 1024 * i);
     }
   };
 

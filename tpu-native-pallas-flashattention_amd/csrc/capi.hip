@@ -978,8 +978,8 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   p->dma = a->page_size % rows_per_load == 0 &&
            (int64_t)a->num_pages * a->page_size <= (int64_t)0xffffffff / a->num_kv_heads &&
            (((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0;
-  // own_stream: at most 8 heads, whole rows of a kernel's head dim, whole page groups
-  p->thin = p->dma && p->g <= 8 && a->head_dim == *D && a->page_size % std::max(4, rows_per_load) == 0 &&
+  // own_stream: at most 8 heads, whole page groups
+  p->thin = p->dma && p->g <= 8 && a->page_size % std::max(4, rows_per_load) == 0 &&
             ((uintptr_t)a->q & 15) == 0;
   if (a->batch > 0) plan_prefix(p, *D, a->dtype == PF_DTYPE_F32 ? 4 : 2);
   const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
