@@ -158,6 +158,15 @@ def test_work_lists(dt, batch, hq, hkv, d, page, prefix, hi):
     check(make(dt, batch, hq, hkv, d, page, prefix, lens, poison=False), dt)
 
 
+@pytest.mark.parametrize("page", [17, 18, 31, 50, 100])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (20, 2)])
+@pytest.mark.parametrize("dt,d", [("bf16", 64), ("f16", 128), ("bf16", 256), ("bf16", 80), ("f32", 64), ("f32", 128),
+                                  ("f32", 36)])
+def test_pages_that_a_stage_straddles(dt, d, hq, hkv, page):
+    note(f"prefix {dt} {hq}/{hkv} D={d} page={page}")
+    check(make(dt, 6, hq, hkv, d, page, 333, [0, 1, page, 15 * page + 3, 16, 200]), dt)
+
+
 @pytest.mark.parametrize("dt,batch,hq,hkv,d,page,prefix,lens", [
     ("bf16", 1, 4, 1, 128, 16, 0, [30000]),        # one sequence over every wave
     ("f16", 1, 20, 1, 64, 16, 77, [30000]),        # ... over every workgroup
@@ -262,6 +271,18 @@ def test_pools_past_32_bits(page):
     assert torch.equal(kf[far:], k) and torch.equal(vf[far:], v)
     near = check((q, k, v, ptab, prefix, table, lens), "bf16")
     assert torch.equal(near, paged_flash_attention_prefix(q, kf, vf, move(ptab), prefix, move(table), lens))
+
+
+@pytest.mark.parametrize("page", [20, 50])
+def test_straddled_pages_past_32_bits(page):
+    """Past 4 GiB a pool's pages are not picked by the lane: the attention within its bound all the same."""
+    q, k, v, ptab, prefix, table, lens = make("bf16", 3, 8, 2, 128, page, 200, [30, 0, 55], poison=False)
+    want, bound = reference(q, k, v, ptab, prefix, table, lens)
+    far = (1 << 32) // k[0].numel() + 3
+    kf, vf = (torch.empty(far + x.shape[0], *x.shape[1:], dtype=x.dtype, device="cuda") for x in (k, v))
+    kf[far:], vf[far:] = k, v
+    got = paged_flash_attention_prefix(q, kf, vf, ptab + far, prefix, torch.where(table < 0, table, table + far), lens)
+    assert ((got.double() - want).abs() <= bound + torch.finfo(q.dtype).eps / 2 * (want.abs() + bound)).all()
 
 
 def test_prefix_length_on_the_device_captured():

@@ -26,10 +26,11 @@
 // many tiles (two of K, two of V): a second barrier, in the middle of a block,
 // frees K_{t+1}'s tile for K_{t+3} while P.V of block t runs, and a wait is for the
 // tile needed next alone. The tiles come by direct global -> LDS loads of whole
-// rows (1 KB each, inside one page; rows past the length and columns past the
-// stored head dim lie outside the load's buffer range and arrive as zeros). Pages
-// that such loads would straddle and unaligned pools are staged through registers
-// instead.
+// rows (1 KB each; rows past the length and columns past the stored head dim lie
+// outside the load's buffer range and arrive as zeros), one page lookup per wave
+// and tile, two where 16 rows may straddle pages (50-row pages, 64 sequences of up
+// to 2048 keys over 4000: 75 us, staged through registers 241). Small odd pages,
+// such pools past 4 GiB and unaligned ones are staged through registers.
 // Measured (bfloat16, head_dim 128, 32 heads over 8, 128 sequences, 32768 prefix
 // keys): the prefix alone 94 us with an item per CU, 90 (764 TFLOP/s) with two. One
 // wave a SIMD leaves the pipeline bound by its instructions and their latencies;
@@ -40,8 +41,8 @@
 // products that share the SIMDs. 32 sequences over 6000 keys: 31 us.
 //
 // Own keys with at most 8 heads a KV head: the workgroup's waves each stream a
-// run of their own (own_stream). More heads, odd pages and unaligned operands: the
-// workgroup runs the prefix
+// run of their own (own_stream). More heads, small odd pages and unaligned
+// operands: the workgroup runs the prefix
 // items' pipeline over its run, across the sequences: the block after a
 // sequence's last one is the next sequence's first.
 #pragma once
@@ -59,6 +60,7 @@ constexpr int kBN = 64;      // keys per block
 constexpr int kRows = kPrefixRows;
 
 constexpr uint32_t kPastRange = 0x7ffffff0u;  // an offset past any load's buffer range
+constexpr uint32_t kPastPool = 0xfffffff0u;   // ... past any pool below 4 GiB
 constexpr int kPG = 2;  // the work list's lengths are those of a paged call
 using stream::Cursor;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
@@ -90,16 +92,18 @@ __device__ inline void own_note(const PrefixParams& p, const stream::Partition& 
 // Wave w loads rows 16 w .. 16 w + 15. DMA > 0: whole rows by direct loads; 16:
 // the wave's rows lie in one page (page_size % 16 == 0), so that a tile takes one
 // lookup and one descriptor -- with a wave on each SIMD the scalar instructions of
-// one per load cost as much as the exponentials; 1: each load's rows do. DMA = 0:
-// every lane fetches its 16-byte chunks itself.
+// one per load cost as much as the exponentials; 2: they lie in at most two pages
+// (page_size >= 16), and each lane picks its row's, by offsets in the whole pool
+// (below 4 GiB); 1: each load's rows lie in one page. DMA = 0: every lane fetches
+// its 16-byte chunks itself.
 template <typename T, int D, int DMA>
 struct PageTiles {
   using G = Tile<T, D>;
   static constexpr int PT = G::CPR / 4;          // loads per lane and tile
   static constexpr int RPL = 1024 / G::RB;       // rows per load
-  static constexpr int GR = DMA == 16 ? 16 : RPL;  // rows per lookup
-  static constexpr int NG = 16 / GR;             // lookups of a wave per tile
-  uint32_t voff[PT];  // the lane's byte offset within the lookup's rows
+  static constexpr int GR = DMA == 16 ? 16 : DMA == 2 ? 15 : RPL;  // rows from lookup to lookup
+  static constexpr int NG = DMA == 2 ? 2 : 16 / GR;                // lookups of a wave per tile
+  uint32_t voff[PT];  // the lane's byte offset within the lookup's rows (DMA = 2: the wave's)
   uint32_t row0;      // the wave's first row; load u: + RPL u
   uint32_t slot0;     // the wave's LDS byte offset of load 0; load u: + 1024 u
   uint32_t rb;        // stored row bytes
@@ -119,7 +123,7 @@ struct PageTiles {
       const int row = RPL * u + lane / G::CPR;
       const int chunk = (lane % G::CPR) ^ tile_swz<G::CPR>(16 * w + row);
       // columns past the stored row: past any range
-      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)((row % GR * p.dr + chunk * G::EPC) * G::ES) : kPastRange;
+      voff[u] = chunk * G::EPC < p.dr ? (uint32_t)(((DMA == 2 ? row : row % GR) * p.dr + chunk * G::EPC) * G::ES) : kPastRange;
     }
   }
   __device__ inline int kv_head(const Cursor& c) const { return n_hc == 1 ? c.j : c.j / n_hc; }
@@ -141,6 +145,8 @@ struct PageTiles {
     return x;
   }
   // The byte offsets in the pool where they start, and the valid bytes behind them.
+  // (DMA = 2: those of the wave's first row as if it lay in either page, modulo
+  // 2^32, and the valid rows and those in the first page.)
   struct Rows {
     uint64_t at[NG];
     uint32_t bytes[NG];
@@ -151,17 +157,31 @@ struct PageTiles {
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const int key = key_of(c, u), id = min(max(page.id[u], 0), p.num_pages - 1);
+      if constexpr (DMA == 2) {
+        const int key0 = key_of(c, 0), first = logical(key) * p.page_size;
+        x.at[u] = (((uint32_t)id * p.Hkv + kvh) * p.page_size + (uint32_t)(key0 - first)) * rb;
+        x.bytes[u] = u == 0 ? min(max(c.L - key0, 0), 16) : logical(key0) * p.page_size + p.page_size - key0;
+        continue;
+      }
       x.at[u] = (uint64_t)(((uint32_t)id * p.Hkv + kvh) * p.page_size + (key - logical(key) * p.page_size)) * rb;
       x.bytes[u] = min(max(c.L - key, 0), GR) * rb;
     }
     return x;
   }
-  // The descriptor of the wave's rows (DMA = 16), for all its loads.
+  // The descriptor of the wave's rows (DMA = 16; 2: of the pool), for all its loads.
   __device__ inline i32x4 rows_desc(const void* pool, const Rows& x) const {
+    if constexpr (DMA == 2)
+      return dma_pin(make_desc(pool, (uint32_t)p.num_pages * p.Hkv * p.page_size * rb));
     return dma_pin(make_desc(static_cast<const char*>(pool) + x.at[0], x.bytes[0]));
   }
-  __device__ inline void load(const i32x4& pinned, int u, char* tile) const {
-    dma16_pinned<true>(pinned, voff[u], __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 1024 * u));
+  __device__ inline void load(const i32x4& pinned, const Rows& x, int u, char* tile) const {
+    uint32_t at = voff[u];
+    if constexpr (DMA == 2) {
+      const uint32_t row = RPL * u + lane / G::CPR;
+      at += row < x.bytes[1] ? (uint32_t)x.at[0] : (uint32_t)x.at[1];
+      if (row >= x.bytes[0] || voff[u] == kPastRange) at = kPastPool;
+    }
+    dma16_pinned<true>(pinned, at, __builtin_amdgcn_readfirstlane(lds_u32(tile) + slot0 + 1024 * u));
   }
   __device__ inline void load(const void* pool, const Rows& x, int u, char* tile) const {
     const i32x4 d = make_desc(static_cast<const char*>(pool) + x.at[u], x.bytes[u]);
@@ -197,10 +217,12 @@ struct PageTiles {
 // (Half of that, refilled stage by stage, or the prefix pipeline over 64-key
 // blocks, is what leaves a CU that also computes a prefix item short of memory
 // traffic.) A sequence's query rows come the same way, with its first stage.
-// PG: rows of one page lookup (page_size % PG == 0).
+// PG: rows of one page lookup (page_size % PG == 0); kSplit: a stage lies in at
+// most two pages and each lane picks its row's, as PageTiles with DMA = 2.
 // ---------------------------------------------------------------------------
 constexpr int kOwnKeys = 16;   // keys per stage
 constexpr int kOwnHeads = 8;   // query rows per sequence, at most
+constexpr int kSplit = 2;
 
 template <typename T, int D>
 struct OwnGeo {
@@ -231,8 +253,9 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   using G = OwnGeo<T, D>;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int SK = kOwnKeys, RB = G::RB, NL = G::NL, NSTEP = G::CPR / 4, NACC = D / 16;
-  constexpr int kGroups = SK / PG, kPer = NL / kGroups;
-  static_assert(PG % G::RPL == 0 && SK % PG == 0, "a page group is whole loads of one stage");
+  constexpr bool SPLIT = PG == kSplit;
+  constexpr int kGroups = SPLIT ? 2 : SK / PG, kPer = SPLIT ? NL : NL / kGroups;
+  static_assert(SPLIT || (PG % G::RPL == 0 && SK % PG == 0), "a page group is whole loads of one stage");
   const DecodeParams& own = p.own;
   const int lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
   const int g = p.g, J = p.Hkv, ps = p.page_size;
@@ -255,16 +278,30 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   for (int i = 0; i < NL; ++i) {
     const int row = G::RPL * i + lane / G::CPR;
     const uint32_t at = 16 * ((lane % G::CPR) ^ G::swz(row));
-    loff[i] = at < rb ? row % PG * rb + at : kPastRange;
+    loff[i] = at < rb ? (SPLIT ? row : row % PG) * rb + at : kPastRange;
   }
   // A stage's page groups: pool row and valid rows of each. Groups past the
-  // length load nothing and look nothing up (-1 padding).
+  // length load nothing and look nothing up (-1 padding). SPLIT: the pool row of
+  // the stage's first key as if it lay in the page of the first, or the last, valid
+  // key (modulo 2^32); its valid keys and those in the first page.
   struct Stage {
     uint32_t row[kGroups];
     int valid[kGroups];
   };
   auto look = [&](const Cursor& c) {
     Stage s;
+    if constexpr (SPLIT) {
+      const int key0 = c.st * SK, n = min(c.L - key0, SK);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int lp = fast_div(i == 0 ? key0 : key0 + n - 1, p.div_page);
+        int page = stream::sload_i32(own.block_tables, (int64_t)c.b * own.pages_per_seq + lp);
+        page = min(max(page, 0), p.num_pages - 1);
+        s.row[i] = ((uint32_t)page * p.Hkv + c.j) * ps + (uint32_t)(key0 - lp * ps);
+        s.valid[i] = i == 0 ? n : (int)fast_div(key0, p.div_page) * ps + ps - key0;
+      }
+      return s;
+    }
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const int key = c.st * SK + i * PG;
@@ -278,6 +315,17 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   };
   auto load = [&](const void* pool, const Stage& s, char* tile) {
     const uint32_t at = lds_u32(tile);
+    if constexpr (SPLIT) {
+      const i32x4 d = dma_pin(make_desc(pool, (uint32_t)p.num_pages * p.Hkv * ps * rb));
+      const uint32_t r0 = s.row[0] * rb, r1 = s.row[1] * rb;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int row = G::RPL * i + lane / G::CPR;
+        const uint32_t off = loff[i] + (row < s.valid[1] ? r0 : r1);
+        dma16_pinned<true>(d, row < s.valid[0] && loff[i] != kPastRange ? off : kPastPool, at + 1024 * i);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const i32x4 d = make_desc(static_cast<const char*>(pool) + (uint64_t)s.row[i] * rb, s.valid[i] * rb);
@@ -511,10 +559,10 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   typename PTiles::Rows r1, r2, r3;
   typename PTiles::Pages next;
   auto whole = [&](const void* pool, [[maybe_unused]] const Cursor& c, const typename PTiles::Rows& x, char* tile) {
-    if constexpr (DMA == 16) {
+    if constexpr (DMA > 1) {
       const i32x4 d = tiles.rows_desc(pool, x);
 #pragma unroll
-      for (int u = 0; u < PT; ++u) tiles.load(d, u, tile);
+      for (int u = 0; u < PT; ++u) tiles.load(d, x, u, tile);
     } else if constexpr (DMA > 0) {
 #pragma unroll
       for (int u = 0; u < PT; ++u) tiles.load(pool, x, u, tile);
@@ -543,18 +591,18 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   auto vdst = [&](auto par) { return vbuf + (1 - decltype(par)::value) * G::BYTES; };
   i32x4 vd, kd;
   auto begin = [&](auto par) __attribute__((always_inline)) {
-    if constexpr (DMA == 16) {
+    if constexpr (DMA > 1) {
       vd = tiles.rows_desc(p.v, r1);
       kd = tiles.rows_desc(p.k, r3);
     }
     if constexpr (DMA == 0) tiles.copy(p.v, cs, vdst(par));
   };
   auto v_part = [&](int i, auto par) __attribute__((always_inline)) {
-    if constexpr (DMA == 16) tiles.load(vd, i, vdst(par));
+    if constexpr (DMA > 1) tiles.load(vd, r1, i, vdst(par));
     else if constexpr (DMA > 0) tiles.load(p.v, r1, i, vdst(par));
   };
   auto k_part = [&](int i, auto par) __attribute__((always_inline)) {
-    if constexpr (DMA == 16) tiles.load(kd, i, kcur(par));
+    if constexpr (DMA > 1) tiles.load(kd, r3, i, kcur(par));
     else if constexpr (DMA > 0) tiles.load(p.k, r3, i, kcur(par));
   };
   // The middle: V_t is there (after it K_{t+2} and V_{t+1} were asked for), and
@@ -974,7 +1022,8 @@ template <typename T, int D>
 hipError_t launch_pages(const PrefixParams& p, hipStream_t st) {
   if (!p.dma) return launch<T, D, 0, 0>(p, st);
   constexpr int PG = OwnGeo<T, D>::RPL == 8 ? 8 : 4;
-  if (p.page_size % 16 == 0) return p.thin ? launch<T, D, 16, 16>(p, st) : launch<T, D, 16, 0>(p, st);
+  if (p.dma == 16) return p.thin ? launch<T, D, 16, 16>(p, st) : launch<T, D, 16, 0>(p, st);
+  if (p.dma == 2) return p.thin ? launch<T, D, 2, kSplit>(p, st) : launch<T, D, 2, 0>(p, st);
   return p.thin ? launch<T, D, 1, PG>(p, st) : launch<T, D, 1, 0>(p, st);
 }
 

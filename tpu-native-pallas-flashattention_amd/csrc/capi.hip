@@ -974,14 +974,17 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   p->own.context_lens = a->context_lens;
   p->own.page_size = a->page_size;
   p->own.pages_per_seq = a->pages_per_seq;
-  const int rows_per_load = 1024 / (*D * (a->dtype == PF_DTYPE_F32 ? 4 : 2));
-  p->dma = a->page_size % rows_per_load == 0 &&
-           (int64_t)a->num_pages * a->page_size <= (int64_t)0xffffffff / a->num_kv_heads &&
-           (((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0;
+  const int es = a->dtype == PF_DTYPE_F32 ? 4 : 2, rows_per_load = 1024 / (*D * es);
+  const uint64_t pool_rows = (uint64_t)a->num_pages * a->page_size * a->num_kv_heads;
+  if ((((uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) == 0 && pool_rows <= 0xffffffff) {
+    if (a->page_size % 16 == 0) p->dma = 16;
+    else if (a->page_size >= 16 && pool_rows <= 0xffffffe0u / (a->head_dim * es)) p->dma = 2;
+    else if (a->page_size % rows_per_load == 0) p->dma = 1;
+  }
   // own_stream: at most 8 heads, whole page groups
-  p->thin = p->dma && p->g <= 8 && a->page_size % std::max(4, rows_per_load) == 0 &&
+  p->thin = p->dma && p->g <= 8 && (p->dma > 1 || a->page_size % std::max(4, rows_per_load) == 0) &&
             ((uintptr_t)a->q & 15) == 0;
-  if (a->batch > 0) plan_prefix(p, *D, a->dtype == PF_DTYPE_F32 ? 4 : 2);
+  if (a->batch > 0) plan_prefix(p, *D, es);
   const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
   if (n_pre + p->own.n_waves > kMaxGrid) return PF_ERR_UNSUPPORTED;
   p->n_pre = (int)n_pre;

@@ -348,7 +348,7 @@ struct PrefixParams {
   int dr;                // stored head dim
   int num_pages, page_size;
   FastDiv div_page;
-  int dma;         // whole loads lie inside a page and the pools are aligned
+  int dma;         // direct loads: 16 rows lie in one page (16) or at most two (2), or those of 1 KB in one (1); 0: none
   float scale_log2;
   // the prefix
   const int32_t* table;    // [pages]
