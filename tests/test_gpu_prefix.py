@@ -158,8 +158,19 @@ def test_work_lists(dt, batch, hq, hkv, d, page, prefix, hi):
     check(make(dt, batch, hq, hkv, d, page, prefix, lens, poison=False), dt)
 
 
+@pytest.mark.parametrize("dt,hq,hkv,d,page", [("bf16", 32, 2, 128, 16), ("f16", 18, 2, 64, 32), ("f32", 8, 2, 64, 20),
+                                              ("bf16", 24, 2, 256, 16), ("f32", 13, 1, 128, 4)])
+def test_runs_of_short_sequences(dt, hq, hkv, d, page):
+    """A wave's run of several sequences of one stage, and of one and two and three."""
+    rng = np.random.default_rng(5)
+    lens = rng.integers(0, 17, 1400).tolist()
+    lens[700:] = rng.integers(0, 40, 700).tolist()
+    note(f"prefix {dt} {hq}/{hkv} D={d} page={page} short sequences")
+    check(make(dt, 1400, hq, hkv, d, page, 40, lens, poison=False), dt)
+
+
 @pytest.mark.parametrize("page", [17, 18, 31, 50, 100])
-@pytest.mark.parametrize("hq,hkv", [(8, 2), (20, 2)])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (20, 2), (36, 2)])
 @pytest.mark.parametrize("dt,d", [("bf16", 64), ("f16", 128), ("bf16", 256), ("bf16", 80), ("f32", 64), ("f32", 128),
                                   ("f32", 36)])
 def test_pages_that_a_stage_straddles(dt, d, hq, hkv, page):

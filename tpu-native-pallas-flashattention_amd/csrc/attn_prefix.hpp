@@ -40,7 +40,7 @@
 // With the own keys (4.3 MB a sequence, 96 us alone, 5.6 TB/s) 136 us: reads beside
 // products that share the SIMDs. 32 sequences over 6000 keys: 31 us.
 //
-// Own keys with at most 8 heads a KV head: the workgroup's waves each stream a
+// Own keys with at most 16 heads a KV head: the workgroup's waves each stream a
 // run of their own (own_stream). More heads, small odd pages and unaligned
 // operands: the workgroup runs the prefix
 // items' pipeline over its run, across the sequences: the block after a
@@ -208,7 +208,7 @@ struct PageTiles {
 };
 
 // ---------------------------------------------------------------------------
-// Own keys, at most 8 query heads per KV head: wave w of own.n_waves streams its
+// Own keys, at most 16 query heads per KV head: wave w of own.n_waves streams its
 // run of the work list in stages of 16 keys through a ring of two stages in LDS,
 // with no barrier: 16x16 MFMAs, S^T (16 keys x heads) and O^T += V^T P^T, as the
 // streaming decode. A stage's K is free once its scores are there, its V once
@@ -216,12 +216,13 @@ struct PageTiles {
 // in flight nearly always, 64 KB of a workgroup's four waves at head_dim 128.
 // (Half of that, refilled stage by stage, or the prefix pipeline over 64-key
 // blocks, is what leaves a CU that also computes a prefix item short of memory
-// traffic.) A sequence's query rows come the same way, with its first stage.
+// traffic.) A sequence's query rows come the same way, with its first stage, or,
+// where those of a one-stage sequence still wait to be taken, right after them.
 // PG: rows of one page lookup (page_size % PG == 0); kSplit: a stage lies in at
 // most two pages and each lane picks its row's, as PageTiles with DMA = 2.
 // ---------------------------------------------------------------------------
 constexpr int kOwnKeys = 16;   // keys per stage
-constexpr int kOwnHeads = 8;   // query rows per sequence, at most
+constexpr int kOwnHeads = 16;  // query rows per sequence, at most
 constexpr int kSplit = 2;
 
 template <typename T, int D>
@@ -232,7 +233,7 @@ struct OwnGeo {
   static constexpr int NL = TILE / 1024;         // loads per tile
   static constexpr int RPL = 1024 / RB;          // rows per load
   static constexpr int QB = kOwnHeads * RB;      // query rows
-  static constexpr int WAVE = 4 * TILE + 2 * QB;  // K, V: two stages each; Q: two sequences
+  static constexpr int WAVE = 4 * TILE + QB;     // K, V: two stages each; Q: one sequence
   static_assert(RB == 128 || RB == 256 || RB == 512, "row sizes");
   // Chunk permutation of row r (XOR of the low bits of the chunk index): the 16
   // rows of a K read hit 16 bank groups (128-byte rows: row bit 0 already parts
@@ -268,7 +269,7 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
 
   char* const kbuf = ring;                 // stages k & 1
   char* const vbuf = ring + 2 * G::TILE;
-  char* const qbuf = ring + 4 * G::TILE;   // sequences in turn
+  char* const qbuf = ring + 4 * G::TILE;
 
   // The chunk that this lane fetches for load i: its byte offset within the page group.
   // (Columns past the stored row: past any range.)
@@ -333,28 +334,36 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
       for (int e = 0; e < kPer; ++e) dma16<true>(d, loff[i * kPer + e], at + 1024 * (i * kPer + e));
     }
   };
-  auto load_q = [&](const Cursor& c, char* q) {
-    const i32x4 d = make_desc(static_cast<const T*>(p.q) + ((int64_t)c.b * p.Hq + (int64_t)c.j * g) * p.dr, g * rb);
+  // q_wait: the queries in qbuf are still to be taken; qb, qj: the sequence whose
+  // queries come after those (qb < 0: none).
+  bool q_wait = false;
+  int qb = -1, qj = 0;
+  auto load_q = [&](int b, int j) {
+    if (q_wait) {
+      qb = b;
+      qj = j;
+      return;
+    }
+    q_wait = true;
+    const i32x4 d = make_desc(static_cast<const T*>(p.q) + ((int64_t)b * p.Hq + (int64_t)j * g) * p.dr, g * rb);
 #pragma unroll
     for (int i = 0; i < G::QB / 1024; ++i) {
       const int row = G::RPL * i + lane / G::CPR;
       const uint32_t at = 16 * ((lane % G::CPR) ^ (row & G::QMASK));
-      dma16(d, at < rb ? row * rb + at : kPastRange, lds_u32(q) + 1024 * i);
+      if (G::RPL * i < g) dma16(d, at < rb ? row * rb + at : kPastRange, lds_u32(qbuf) + 1024 * i);
     }
   };
 
   // Prologue: stages 0 and 1. pc: the stage that is loaded next.
   Cursor pc = cc;
-  int q_in = 0, q_out = 0;  // sequences whose queries were asked for, and taken
-  load_q(cc, qbuf);
-  ++q_in;
+  load_q(cc.b, cc.j);
   Stage st = look(cc);
   load(p.k, st, kbuf);
   load(p.v, st, vbuf);
   stream::cursor_next<kPG, SK>(pc, own, J);
   if (n > 1) {
     st = look(pc);
-    if (pc.st == 0) load_q(pc, qbuf + G::QB * (q_in++ & 1));
+    if (pc.st == 0) load_q(pc.b, pc.j);
     load(p.k, st, kbuf + G::TILE);
     load(p.v, st, vbuf + G::TILE);
     stream::cursor_next<kPG, SK>(pc, own, J);
@@ -393,11 +402,15 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
     char* const sK = kbuf + (k & 1) * G::TILE;
     char* const sV = vbuf + (k & 1) * G::TILE;
     if (k == 0 || cc.st == 0) {
-      const char* sQ = qbuf + G::QB * (q_out++ & 1);
 #pragma unroll
       for (int s = 0; s < NSTEP; ++s)
-        qf[s] = i16 < kOwnHeads ? lds16(sQ + i16 * RB + 16 * ((4 * s + h) ^ (i16 & G::QMASK)))
-                                : (u32x4){0u, 0u, 0u, 0u};
+        qf[s] = i16 < g ? lds16(qbuf + i16 * RB + 16 * ((4 * s + h) ^ (i16 & G::QMASK))) : (u32x4){0u, 0u, 0u, 0u};
+      q_wait = false;
+      if (qb >= 0) {
+        wait_lds();
+        load_q(qb, qj);
+        qb = -1;
+      }
 #pragma unroll
       for (int a = 0; a < NACC; ++a) acc[a] = (f32x4)(0.f);
       m_run = -__FLT_MAX__;
@@ -412,7 +425,7 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
     if (more) {
       st = look(pc);
       wait_lds();  // K and Q are read
-      if (pc.st == 0) load_q(pc, qbuf + G::QB * (q_in++ & 1));
+      if (pc.st == 0) load_q(pc.b, pc.j);
       load(p.k, st, sK);
     }
 

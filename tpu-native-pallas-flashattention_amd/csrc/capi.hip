@@ -981,8 +981,8 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
     else if (a->page_size >= 16 && pool_rows <= 0xffffffe0u / (a->head_dim * es)) p->dma = 2;
     else if (a->page_size % rows_per_load == 0) p->dma = 1;
   }
-  // own_stream: at most 8 heads, whole page groups
-  p->thin = p->dma && p->g <= 8 && (p->dma > 1 || a->page_size % std::max(4, rows_per_load) == 0) &&
+  // own_stream: at most 16 heads, whole page groups
+  p->thin = p->dma && p->g <= 16 && (p->dma > 1 || a->page_size % std::max(4, rows_per_load) == 0) &&
             ((uintptr_t)a->q & 15) == 0;
   if (a->batch > 0) plan_prefix(p, *D, es);
   const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
