@@ -37,11 +37,13 @@
 // what helped was one lookup and descriptor per tile and wave, tile addresses that
 // are constants of each block's copy, nothing of the own keys' code in the loop (177
 // us for prefix and own keys -> 144), and page lookups a block ahead (142 -> 136).
+// float32 with at most 128 rows a KV head streams the prefix as the own keys, 16
+// rows a wave (plan_prefix has the figures).
 // With the own keys (4.3 MB a sequence, 96 us alone, 5.6 TB/s) 136 us: reads beside
 // products that share the SIMDs. 32 sequences over 6000 keys: 31 us.
 //
 // Own keys with at most 16 heads a KV head: the workgroup's waves each stream a
-// run of their own (own_stream). More heads, small odd pages and unaligned
+// run of their own (key_stream). More heads, small odd pages and unaligned
 // operands: the workgroup runs the prefix
 // items' pipeline over its run, across the sequences: the block after a
 // sequence's last one is the next sequence's first.
@@ -248,8 +250,10 @@ struct OwnGeo {
 // The wave's LDS reads so far have their data (what they read may be overwritten).
 __device__ inline void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
-template <typename T, int D, int PG>
-__device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, int w) {
+// PRE (float32, few rows): w's item of the prefix instead, 16 of a KV head's rows
+// against one chunk of its keys.
+template <typename T, int D, int PG, bool PRE>
+__device__ __forceinline__ void key_stream(const PrefixParams& p, char* ring, int w) {
   using MF = stream::Mfma16<T>;
   using G = OwnGeo<T, D>;
   constexpr bool F32 = sizeof(T) == 4;
@@ -259,13 +263,38 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   static_assert(SPLIT || (PG % G::RPL == 0 && SK % PG == 0), "a page group is whole loads of one stage");
   const DecodeParams& own = p.own;
   const int lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
-  const int g = p.g, J = p.Hkv, ps = p.page_size;
+  const int J = p.Hkv, ps = p.page_size;
+  const int32_t* const table = PRE ? p.table : own.block_tables;
+  const int pages = PRE ? p.pages : own.pages_per_seq;
 
-  if (w >= own.n_waves) return;
   Cursor cc;
-  stream::Partition part((int64_t)0, (int64_t)0);
-  const int64_t n = stream::wave_plan<kPG, SK>(own, J, own.n_waves, w, &cc, &part);
+  [[maybe_unused]] stream::Partition part((int64_t)0, (int64_t)0);
+  int64_t n;
+  int r0 = 0, piece = 0;  // PRE: the item's first row, and its chunk
+  if constexpr (PRE) {
+    // The waves of a workgroup: row groups, then chunks of one KV head, which is
+    // the workgroups' innermost index.
+    const int wg = w >> 2, kvh = wg % J, y = 4 * (wg / J) + (w & 3);
+    piece = y / p.n_tiles;
+    r0 = kOwnHeads * (y - piece * p.n_tiles);
+    const int key0 = piece * p.chunk, L = piece < p.n_split ? min(prefix_len(p), key0 + p.chunk) : 0;
+    n = (L - key0 + SK - 1) / SK;
+    cc = Cursor{0, kvh, key0 / SK, key0 / SK + (int)n, L};
+  } else {
+    if (w >= own.n_waves) return;
+    n = stream::wave_plan<kPG, SK>(own, J, own.n_waves, w, &cc, &part);
+  }
   if (n <= 0) return;
+  const int g = PRE ? min(p.rows - r0, kOwnHeads) : p.g;  // query rows
+  auto next = [&](Cursor& c) {
+    if constexpr (PRE) ++c.st;
+    else stream::cursor_next<kPG, SK>(c, own, J);
+  };
+  // PRE: the (batch, head) of the item's row.
+  auto head_of = [&](int row) {
+    const int b = (r0 + row) / p.g;
+    return b * p.Hq + cc.j * p.g + (r0 + row - b * p.g);
+  };
 
   char* const kbuf = ring;                 // stages k & 1
   char* const vbuf = ring + 2 * G::TILE;
@@ -296,7 +325,7 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int lp = fast_div(i == 0 ? key0 : key0 + n - 1, p.div_page);
-        int page = stream::sload_i32(own.block_tables, (int64_t)c.b * own.pages_per_seq + lp);
+        int page = stream::sload_i32(table, (int64_t)c.b * pages + lp);
         page = min(max(page, 0), p.num_pages - 1);
         s.row[i] = ((uint32_t)page * p.Hkv + c.j) * ps + (uint32_t)(key0 - lp * ps);
         s.valid[i] = i == 0 ? n : (int)fast_div(key0, p.div_page) * ps + ps - key0;
@@ -308,7 +337,7 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
       const int key = c.st * SK + i * PG;
       s.valid[i] = min(max(c.L - key, 0), PG);
       const int lp = s.valid[i] > 0 ? (int)fast_div(key, p.div_page) : 0;
-      int page = s.valid[i] > 0 ? stream::sload_i32(own.block_tables, (int64_t)c.b * own.pages_per_seq + lp) : 0;
+      int page = s.valid[i] > 0 ? stream::sload_i32(table, (int64_t)c.b * pages + lp) : 0;
       page = min(max(page, 0), p.num_pages - 1);
       s.row[i] = ((uint32_t)page * p.Hkv + c.j) * ps + (s.valid[i] > 0 ? key - lp * ps : 0);
     }
@@ -345,12 +374,14 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
       return;
     }
     q_wait = true;
-    const i32x4 d = make_desc(static_cast<const T*>(p.q) + ((int64_t)b * p.Hq + (int64_t)j * g) * p.dr, g * rb);
+    const i32x4 d = PRE ? make_desc(p.q, (uint32_t)own.B * p.Hq * rb)
+                        : make_desc(static_cast<const T*>(p.q) + ((int64_t)b * p.Hq + (int64_t)j * g) * p.dr, g * rb);
 #pragma unroll
     for (int i = 0; i < G::QB / 1024; ++i) {
       const int row = G::RPL * i + lane / G::CPR;
       const uint32_t at = 16 * ((lane % G::CPR) ^ (row & G::QMASK));
-      if (G::RPL * i < g) dma16(d, at < rb ? row * rb + at : kPastRange, lds_u32(qbuf) + 1024 * i);
+      const bool on = at < rb && (!PRE || row < g);
+      if (G::RPL * i < g) dma16(d, on ? (PRE ? head_of(row) : row) * rb + at : kPastRange, lds_u32(qbuf) + 1024 * i);
     }
   };
 
@@ -360,13 +391,13 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
   Stage st = look(cc);
   load(p.k, st, kbuf);
   load(p.v, st, vbuf);
-  stream::cursor_next<kPG, SK>(pc, own, J);
+  next(pc);
   if (n > 1) {
     st = look(pc);
-    if (pc.st == 0) load_q(pc.b, pc.j);
+    if (!PRE && pc.st == 0) load_q(pc.b, pc.j);
     load(p.k, st, kbuf + G::TILE);
     load(p.v, st, vbuf + G::TILE);
-    stream::cursor_next<kPG, SK>(pc, own, J);
+    next(pc);
   }
 
   // LDS read offsets. K (A operand of S^T): row i16, chunk 4s + h; past 16 chunks
@@ -401,7 +432,7 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
     else wait_vm<0>();
     char* const sK = kbuf + (k & 1) * G::TILE;
     char* const sV = vbuf + (k & 1) * G::TILE;
-    if (k == 0 || cc.st == 0) {
+    if (k == 0 || (!PRE && cc.st == 0)) {
 #pragma unroll
       for (int s = 0; s < NSTEP; ++s)
         qf[s] = i16 < g ? lds16(qbuf + i16 * RB + 16 * ((4 * s + h) ^ (i16 & G::QMASK))) : (u32x4){0u, 0u, 0u, 0u};
@@ -425,7 +456,7 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
     if (more) {
       st = look(pc);
       wait_lds();  // K and Q are read
-      if (pc.st == 0) load_q(pc.b, pc.j);
+      if (!PRE && pc.st == 0) load_q(pc.b, pc.j);
       load(p.k, st, sK);
     }
 
@@ -472,18 +503,23 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
     if (more) {
       wait_lds();  // V is read
       load(p.v, st, sV);
-      stream::cursor_next<kPG, SK>(pc, own, J);
+      next(pc);
     }
 
-    if (cc.st == cc.nst - 1 || k == n - 1) {
+    if ((!PRE && cc.st == cc.nst - 1) || k == n - 1) {
       float l_tot = l_run + __shfl_xor(l_run, 16);
       l_tot = wave_xor32_sum(l_tot);
       if (i16 < g) {
-        const bool whole = piece_st0 == 0 && cc.st == cc.nst - 1;
-        const int64_t seq = (int64_t)cc.b * J + cc.j;
-        if (piece_st0 == 0 && lane == 0) own_note(p, part, w, seq, cc, !first_piece);
-        const int64_t at = own_slot(own, J, w, seq, whole, !first_piece) * g + i16;
-        float* po = own.part_o + at * D;
+        int64_t at;
+        if constexpr (PRE) {
+          at = (int64_t)piece * own.B * p.Hq + head_of(i16);
+        } else {
+          const bool whole = piece_st0 == 0 && cc.st == cc.nst - 1;
+          const int64_t seq = (int64_t)cc.b * J + cc.j;
+          if (piece_st0 == 0 && lane == 0) own_note(p, part, w, seq, cc, !first_piece);
+          at = own_slot(own, J, w, seq, whole, !first_piece) * g + i16;
+        }
+        float* po = (PRE ? p.part_o : own.part_o) + at * D;
 #pragma unroll
         for (int q = 0; q < NACC; ++q) {
           if constexpr (F32) {
@@ -494,11 +530,11 @@ __device__ __forceinline__ void own_stream(const PrefixParams& p, char* ring, in
             *reinterpret_cast<f32x4*>(po + 16 * q + 4 * h) = acc[q];
           }
         }
-        if (h == 0) *reinterpret_cast<f32x2*>(own.part_ml + 2 * at) = (f32x2){m_run, l_tot};
+        if (h == 0) *reinterpret_cast<f32x2*>((PRE ? p.part_ml : own.part_ml) + 2 * at) = (f32x2){m_run, l_tot};
       }
       first_piece = false;
     }
-    stream::cursor_next<kPG, SK>(cc, own, J);
+    next(cc);
   }
 }
 
@@ -887,7 +923,7 @@ __device__ __forceinline__ void run_blocks(const PrefixParams& p, char* smem, in
   finish(cp);
 }
 
-// PG > 0: own keys by own_stream; 0: by the block pipeline.
+// PG > 0: own keys by key_stream; 0: by the block pipeline.
 // The own pipeline needs the registers of two workgroups per CU at most.
 template <typename T, int D, int DMA, int PG>
 __global__ __launch_bounds__(256, (PG == 0 && kFwdWgPerCu<T, D> > 2 ? 2 : kFwdWgPerCu<T, D>))
@@ -896,12 +932,16 @@ void pf_prefix_kernel(PrefixParams p) {
   static_assert(4 * G::WAVE >= 4 * Tile<T, D>::BYTES, "the waves' rings hold the tiles");
   __shared__ __attribute__((aligned(1024))) char smem[PG > 0 ? 4 * G::WAVE : 4 * Tile<T, D>::BYTES];
   const int item = blockIdx.x - p.n_pre;
+  if constexpr (PG > 0) {
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* const ring = smem + wv * G::WAVE;
+    if (item >= 0) return key_stream<T, D, PG, false>(p, ring, 4 * item + wv);
+    if constexpr (sizeof(T) == 4)
+      if (p.few) return key_stream<T, D, PG, true>(p, ring, 4 * blockIdx.x + wv);
+  }
   if (item < 0) {
     run_blocks<T, D, DMA, false>(p, smem, blockIdx.x);
-  } else if constexpr (PG > 0) {
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    own_stream<T, D, PG>(p, smem + wv * G::WAVE, 4 * item + wv);
-  } else {
+  } else if constexpr (PG == 0) {
     run_blocks<T, D, DMA, true>(p, smem, item);
   }
 }

@@ -899,7 +899,19 @@ int own_waves(const pf::PrefixParams& p, bool thin) {
 // (float16, head_dim 256, 16 sequences over 5003 keys: one after the other 30.6 us,
 // half and half 26; 128 over 16384: 205, 174; 16 over 40000, nearly all of it the
 // prefix's: 70, 88, in proportion 67.)
-void plan_prefix(pf::PrefixParams* p, int D, int es) {
+//
+// float32, at most 128 rows: an item is a wave of 16 rows (few). The matrix cores'
+// float32 rate bounds these, and a workgroup's block takes 32 rows a wave, whatever
+// there are (8 rows of head_dim 128 over 20000 keys: 105 us, 36 as streams; 32 over
+// 8000: 40, 24; 128 over 4000: 53, 48). In 16 bits the blocks wait for memory, and
+// row groups that stream the same keys ask for them twice (64 rows over 60000: 32
+// us, 49; 8 over 20000: 23, 24).
+//
+// Returns the prefix's workgroups.
+int64_t plan_prefix(pf::PrefixParams* p, int D, int es) {
+  constexpr int kFew = 16;  // query rows of a wave
+  p->few = es == 4 && p->thin && p->rows <= pf::kPrefixRows && (int64_t)p->own.B * p->Hq * p->dr * es <= 0x7fffffe0;
+  p->n_tiles = (p->rows + (p->few ? kFew : pf::kPrefixRows) - 1) / (p->few ? kFew : pf::kPrefixRows);
   const int64_t items = (int64_t)p->n_tiles * p->Hkv;
   const bool one = D * es >= 512;
   const auto keys = [&](int64_t c) {  // per chunk, for an item on each of c CUs
@@ -908,15 +920,19 @@ void plan_prefix(pf::PrefixParams* p, int D, int es) {
   };
   // Work per KV head. A prefix key of up to 128 rows costs an own key's time in 16
   // bits, three times that in float32; own keys: half their bound.
-  const double pre = (double)p->n_tiles * p->len * (es == 4 ? 3 : 1);
+  const double pre = (double)p->n_tiles * p->len * (es == 4 && !p->few ? 3 : 1);
   const double own = 0.5 * p->own.B * p->n_hc * (double)p->own.pages_per_seq * p->page_size;
   int64_t cus = kCus;  // the prefix's
   if (one) {
     if (own > 0) cus = std::min<int64_t>(kCus - 8, std::max<int64_t>(kCus / 2, (int64_t)(kCus * (pre / (pre + own)))));
-  } else if (pre > 4 * own && keys(2 * kCus) >= 1024) {
+  } else if (!p->few && pre > 4 * own && keys(2 * kCus) >= 1024) {
     cus = 2 * kCus;
   }
-  if (p->len > 0) {
+  if (p->len > 0 && p->few) {
+    const int64_t n = std::max<int64_t>(1, 4 * cus / items);
+    p->chunk = (int)std::max<int64_t>(64, ((p->len + n - 1) / n + 15) / 16 * 16);
+    p->n_split = (p->len + p->chunk - 1) / p->chunk;
+  } else if (p->len > 0) {
     p->chunk = (int)std::max<int64_t>(64, keys(cus));
     if (!one) {
       const int64_t rows3 = 3 * std::min(p->rows, pf::kPrefixRows) / 64 * 64;
@@ -924,11 +940,13 @@ void plan_prefix(pf::PrefixParams* p, int D, int es) {
     }
     p->n_split = (p->len + p->chunk - 1) / p->chunk;
   }
-  p->own_cus = one ? (int)std::max<int64_t>(kCus - cus, kCus - items * p->n_split) : kCus;
+  const int64_t n_pre = p->few ? (int64_t)p->Hkv * (((int64_t)p->n_tiles * p->n_split + 3) / 4) : items * p->n_split;
+  p->own_cus = one ? (int)std::max<int64_t>(kCus - cus, kCus - n_pre) : kCus;
   p->own.n_waves = own_waves(*p, p->thin);
   p->merge_heads = std::min(p->g, 1024 / D);
   while (p->merge_heads > 1 && p->n_split > (int64_t)pf::kMergeLoads * (1024 / D / p->merge_heads))
     p->merge_heads = (p->merge_heads + 1) / 2;
+  return n_pre;
 }
 
 // *D: the compute head dim.
@@ -965,7 +983,6 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   p->len_ptr = a->prefix_len_ptr;
   p->pages = a->prefix_pages;
   p->len = a->prefix_len;
-  p->n_tiles = (p->rows + pf::kPrefixRows - 1) / pf::kPrefixRows;
   p->chunk = 64;
   p->n_hc = (p->g + pf::kPrefixRows - 1) / pf::kPrefixRows;
   p->own_rows = std::min(p->g, pf::kPrefixRows);
@@ -981,11 +998,10 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
     else if (a->page_size >= 16 && pool_rows <= 0xffffffe0u / (a->head_dim * es)) p->dma = 2;
     else if (a->page_size % rows_per_load == 0) p->dma = 1;
   }
-  // own_stream: at most 16 heads, whole page groups
+  // key_stream: at most 16 heads, whole page groups
   p->thin = p->dma && p->g <= 16 && (p->dma > 1 || a->page_size % std::max(4, rows_per_load) == 0) &&
             ((uintptr_t)a->q & 15) == 0;
-  if (a->batch > 0) plan_prefix(p, *D, es);
-  const int64_t n_pre = (int64_t)p->n_tiles * p->Hkv * p->n_split;
+  const int64_t n_pre = a->batch > 0 ? plan_prefix(p, *D, es) : 0;
   if (n_pre + p->own.n_waves > kMaxGrid) return PF_ERR_UNSUPPORTED;
   p->n_pre = (int)n_pre;
   return PF_OK;
@@ -993,18 +1009,23 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
 
 // Rows of the partials: of the prefix's chunks, and of the own pieces (own_slot).
 size_t prefix_rows(const pf::PrefixParams& p) { return (size_t)p.n_split * p.own.B * p.Hq; }
-size_t form_piece_rows(const pf::PrefixParams& p, bool thin) {
-  const size_t seqs = (size_t)p.own.B * p.Hkv * p.n_hc, w = own_waves(p, thin);
+size_t own_piece_rows(const pf::PrefixParams& p) {
+  const size_t seqs = (size_t)p.own.B * p.Hkv * p.n_hc, w = p.own.n_waves;
   return w == 0 ? 0 : (seqs + (seqs <= w ? 1 : 2) * w) * p.own_rows;
 }
-// The own pieces of either form, so that the size does not depend on how the pools
-// are aligned.
-size_t own_piece_rows(const pf::PrefixParams& p) {
-  return std::max(form_piece_rows(p, true), form_piece_rows(p, false));
-}
-size_t prefix_ws(const pf::PrefixParams& p, int D) {
+// The larger of either form's parts, so that the size does not depend on how the
+// operands are aligned.
+size_t prefix_ws(const pf::PrefixParams& p, int D, int es) {
+  size_t pre = 0, own = 0;
+  for (int thin = 0; thin < 2; ++thin) {
+    pf::PrefixParams f = p;
+    f.thin = thin;
+    if (f.own.B > 0) plan_prefix(&f, D, es);
+    pre = std::max(pre, prefix_rows(f));
+    own = std::max(own, own_piece_rows(f));
+  }
   const size_t notes = align256((size_t)p.own.B * p.Hkv * p.n_hc * 8);
-  return std::max<size_t>(partial_bytes(prefix_rows(p), D) + partial_bytes(own_piece_rows(p), D) + notes, 256);
+  return std::max<size_t>(partial_bytes(pre, D) + partial_bytes(own, D) + notes, 256);
 }
 
 }  // namespace
@@ -1012,7 +1033,7 @@ size_t prefix_ws(const pf::PrefixParams& p, int D) {
 size_t pf_paged_prefix_attn_workspace_size(const pf_paged_prefix_attn_args* a) {
   pf::PrefixParams p;
   int D;
-  return fill_prefix(a, &p, &D) == PF_OK ? prefix_ws(p, D) : 0;
+  return fill_prefix(a, &p, &D) == PF_OK ? prefix_ws(p, D, a->dtype == PF_DTYPE_F32 ? 4 : 2) : 0;
 }
 
 int pf_paged_prefix_attn(const pf_paged_prefix_attn_args* a, void* stream) {
@@ -1023,7 +1044,7 @@ int pf_paged_prefix_attn(const pf_paged_prefix_attn_args* a, void* stream) {
   if (a->batch == 0) return PF_OK;
   if (!a->q || !a->k_pages || !a->v_pages || !a->o || !a->context_lens) return PF_ERR_INVALID;
   if ((a->pages_per_seq > 0 && !a->block_tables) || (a->prefix_len > 0 && !a->prefix_table)) return PF_ERR_INVALID;
-  if (!a->workspace || a->workspace_bytes < prefix_ws(p, D) || ((uintptr_t)a->workspace & 255) != 0)
+  if (!a->workspace || a->workspace_bytes < prefix_ws(p, D, a->dtype == PF_DTYPE_F32 ? 4 : 2) || ((uintptr_t)a->workspace & 255) != 0)
     return PF_ERR_WORKSPACE;
   char* ws = static_cast<char*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(ws);

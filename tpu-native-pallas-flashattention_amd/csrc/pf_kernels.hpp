@@ -354,15 +354,16 @@ struct PrefixParams {
   const int32_t* table;    // [pages]
   const int32_t* len_ptr;  // its length in device memory (at most len), or null: len
   int pages, len;
-  int n_tiles;             // ceil(rows / kPrefixRows)
-  int chunk, n_split;      // chunks of `chunk` keys (a multiple of 64)
-  int n_pre;               // work items: n_tiles Hkv n_split
+  int few;                 // float32: items are waves with 16 rows (key_stream), else workgroups with kPrefixRows
+  int n_tiles;             // ceil(rows / an item's)
+  int chunk, n_split;      // chunks of `chunk` keys (a multiple of 64; few: of 16)
+  int n_pre;               // workgroups
   float* part_o;           // [n_split, B, Hq, D]
   float* part_ml;          // [n_split, B, Hq, 2]
   // The sequences' own keys: the streaming decode's work list. Of `own`: B,
   // block_tables, context_lens, page_size, pages_per_seq, n_waves, and the
   // partials, own_rows rows per slot. thin: in stages of 16 keys over n_waves
-  // waves (own_stream); else in blocks of 64 keys over n_waves workgroups.
+  // waves (key_stream); else in blocks of 64 keys over n_waves workgroups.
   DecodeParams own;
   int32_t* own_info;  // [B Hkv n_hc, 2]: where each sequence's pieces are
   int thin;
