@@ -95,3 +95,13 @@ def test_c_workspace_is_bounded(L, dtype, d):
                          prefix_pages=-(-prefix // 16), num_pages=1 << 17, pages_per_seq=64)
                 need = L.pf_paged_prefix_attn_workspace_size(a)
                 assert 0 < need <= (1 << 28) + batch * hq * 64 * (d + 64) * 4, (batch, hq, prefix, need)
+
+
+@pytest.mark.parametrize("dtype,d,page", [(0, 64, 16), (0, 128, 20), (1, 128, 16), (2, 256, 50), (1, 96, 12)])
+@pytest.mark.parametrize("batch,hq,hkv", [(1, 8, 1), (16, 16, 4), (40, 64, 4), (9, 34, 2)])
+def test_c_workspace_wherever_the_operands_lie(L, dtype, d, page, batch, hq, hkv):
+    a = dict(batch=batch, num_heads=hq, num_kv_heads=hkv, head_dim=d, dtype=dtype, page_size=page, prefix_len=5000,
+             prefix_pages=-(-5000 // page), num_pages=4000, pages_per_seq=30)
+    need = L.pf_paged_prefix_attn_workspace_size(args(**a))
+    for over in (dict(q=264), dict(k_pages=264), dict(v_pages=258), dict(q=None, k_pages=None, v_pages=None)):
+        assert L.pf_paged_prefix_attn_workspace_size(args(**a, **over)) == need > 0
