@@ -37,16 +37,15 @@
 // what helped was one lookup and descriptor per tile and wave, tile addresses that
 // are constants of each block's copy, nothing of the own keys' code in the loop (177
 // us for prefix and own keys -> 144), and page lookups a block ahead (142 -> 136).
-// float32 with at most 128 rows a KV head streams the prefix as the own keys, 16
-// rows a wave (plan_prefix has the figures).
 // With the own keys (4.3 MB a sequence, 96 us alone, 5.6 TB/s) 136 us: reads beside
 // products that share the SIMDs. 32 sequences over 6000 keys: 31 us.
 //
 // Own keys with at most 16 heads a KV head: the workgroup's waves each stream a
 // run of their own (key_stream). More heads, small odd pages and unaligned
-// operands: the workgroup runs the prefix
-// items' pipeline over its run, across the sequences: the block after a
-// sequence's last one is the next sequence's first.
+// operands: the workgroup runs the prefix items' pipeline over its run, across the
+// sequences: the block after a sequence's last one is the next sequence's first.
+// float32 with at most 128 rows a KV head streams the prefix like own keys, 16 rows
+// a wave (plan_prefix in capi.hip has the figures).
 #pragma once
 
 #include "decode_stream.hpp"
