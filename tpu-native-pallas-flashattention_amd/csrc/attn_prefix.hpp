@@ -276,7 +276,9 @@ __device__ __forceinline__ void key_stream(const PrefixParams& p, char* ring, in
     const int wg = w >> 2, kvh = wg % J, y = 4 * (wg / J) + (w & 3);
     piece = y / p.n_tiles;
     r0 = kOwnHeads * (y - piece * p.n_tiles);
-    const int key0 = piece * p.chunk, L = piece < p.n_split ? min(prefix_len(p), key0 + p.chunk) : 0;
+    // Waves past the last item have nothing (and a key0 past 32 bits).
+    const bool on = piece < p.n_split;
+    const int key0 = on ? piece * p.chunk : 0, L = on ? min(prefix_len(p), key0 + p.chunk) : 0;
     n = (L - key0 + SK - 1) / SK;
     cc = Cursor{0, kvh, key0 / SK, key0 / SK + (int)n, L};
   } else {
@@ -1000,7 +1002,7 @@ __global__ __launch_bounds__(256) void pf_prefix_merge_kernel(PrefixParams p) {
     M = Mn;
   };
 
-  const int npre = (prefix_len(p) + p.chunk - 1) / p.chunk;
+  const int npre = prefix_chunks(prefix_len(p), p.chunk);
   const int64_t bh = (int64_t)b * p.Hq + kvh * g + h0 + qi;
   auto chunk_row = [&](int s) { return (int64_t)s * p.own.B * p.Hq + bh; };
   fetch(0, npre, p.part_o, p.part_ml, chunk_row);

@@ -931,14 +931,14 @@ int64_t plan_prefix(pf::PrefixParams* p, int D, int es) {
   if (p->len > 0 && p->few) {
     const int64_t n = std::max<int64_t>(1, 4 * cus / items);
     p->chunk = (int)std::max<int64_t>(64, ((p->len + n - 1) / n + 15) / 16 * 16);
-    p->n_split = (p->len + p->chunk - 1) / p->chunk;
+    p->n_split = pf::prefix_chunks(p->len, p->chunk);
   } else if (p->len > 0) {
     p->chunk = (int)std::max<int64_t>(64, keys(cus));
     if (!one) {
       const int64_t rows3 = 3 * std::min(p->rows, pf::kPrefixRows) / 64 * 64;
       p->chunk = (int)std::max<int64_t>(p->chunk, std::min(keys(kCus / 2), rows3));
     }
-    p->n_split = (p->len + p->chunk - 1) / p->chunk;
+    p->n_split = pf::prefix_chunks(p->len, p->chunk);
   }
   const int64_t n_pre = p->few ? (int64_t)p->Hkv * (((int64_t)p->n_tiles * p->n_split + 3) / 4) : items * p->n_split;
   p->own_cus = one ? (int)std::max<int64_t>(kCus - cus, kCus - n_pre) : kCus;

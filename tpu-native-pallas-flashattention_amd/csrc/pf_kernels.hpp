@@ -339,6 +339,9 @@ hipError_t launch_decode_stream(const DecodeParams& p, int dtype, bool paged, hi
 // Attention of a batch over a shared prefix (attn_prefix.hip).
 constexpr int kPrefixRows = 128;  // query rows per workgroup
 constexpr int kMergeLoads = 8;    // partials in flight per lane of the merge
+// Chunks of `chunk` keys that hold len keys. (len + chunk may pass 2^31; every
+// chunk's end, at most 2^17 past len, does not.)
+__host__ __device__ inline int prefix_chunks(int len, int chunk) { return len > 0 ? (len - 1) / chunk + 1 : 0; }
 struct PrefixParams {
   const void* q;  // [B, Hq, dr]
   const void* k;  // page pools
