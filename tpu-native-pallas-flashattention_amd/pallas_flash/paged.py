@@ -144,7 +144,8 @@ def paged_flash_attention_prefix(
 
     Returns:
         ``[batch, num_heads, 1, head_dim]`` in q's dtype. Head dims and dtypes as
-        ``paged_flash_attention``.
+        ``paged_flash_attention``. No gradients: the result has no graph, whatever
+        q and the pools require.
     """
     o = _lib.calls().prefix(q, k_pages, v_pages, prefix_table, prefix_len, block_tables, context_lens, sm_scale)
     if o is not None:
