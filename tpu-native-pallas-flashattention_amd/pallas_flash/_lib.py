@@ -79,7 +79,22 @@ class PagedArgs(ctypes.Structure):
     ]
 
 
-class PagedPrefixArgs(ctypes.Structure):
+class _CountedArgs(ctypes.Structure):
+    """An argument block that refuses numbers past its 32-bit fields, of which
+    ctypes would keep the low bits."""
+
+    def __init_subclass__(cls):
+        cls._counted = [(i, name) for i, (name, kind) in enumerate(cls._fields_) if kind is c_i32]
+
+    def __init__(self, *args, **kwargs):
+        for i, name in self._counted:
+            n = args[i] if i < len(args) else kwargs.get(name, 0)
+            if not -0x80000000 <= n <= 0x7fffffff:
+                raise NotImplementedError(f"{name} = {n} does not fit 32 bits")
+        super().__init__(*args, **kwargs)
+
+
+class PagedPrefixArgs(_CountedArgs):
     _fields_ = [
         ("q", c_ptr), ("k_pages", c_ptr), ("v_pages", c_ptr), ("prefix_table", c_ptr), ("prefix_len_ptr", c_ptr),
         ("block_tables", c_ptr), ("context_lens", c_ptr), ("o", c_ptr),
@@ -119,7 +134,7 @@ class PagedWriteArgs(ctypes.Structure):
 MAX_ROPE_AXES = 4
 
 
-class RopeAxesArgs(ctypes.Structure):
+class RopeAxesArgs(_CountedArgs):
     _fields_ = [
         ("q", c_ptr), ("k", c_ptr), ("q_out", c_ptr), ("k_out", c_ptr),
         ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3),
@@ -131,7 +146,7 @@ class RopeAxesArgs(ctypes.Structure):
     ]
 
 
-class RopePagedWriteArgs(ctypes.Structure):
+class RopePagedWriteArgs(_CountedArgs):
     _fields_ = [
         ("q", c_ptr), ("k", c_ptr), ("v", c_ptr), ("q_out", c_ptr), ("k_pages", c_ptr), ("v_pages", c_ptr),
         ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
