@@ -285,6 +285,15 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def device_ints(t: torch.Tensor, device) -> torch.Tensor:
+    """t in device memory as contiguous int32. Numbers past its range go to the
+    nearest end (a cast would keep their low bits), so that a length, page or
+    position out of bounds stays out of bounds."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-0x80000000, 0x7fffffff)
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 

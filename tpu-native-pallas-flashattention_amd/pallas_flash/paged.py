@@ -184,9 +184,8 @@ def paged_flash_attention_prefix(
         sm_scale = 1.0 / (head_dim ** 0.5)
     _lib.require_device(q, k_pages, v_pages)
     dev = q.device
-    prefix_table, tables, lens = (t.to(device=dev, dtype=torch.int32).contiguous()
-                                  for t in (prefix_table, block_tables, context_lens))
-    len_t = prefix_len.to(device=dev, dtype=torch.int32).reshape(1) if on_device else None
+    prefix_table, tables, lens = (_lib.device_ints(t, dev) for t in (prefix_table, block_tables, context_lens))
+    len_t = _lib.device_ints(prefix_len, dev).reshape(1) if on_device else None
     out_dtype = q.dtype
     cdt = compute_dtype(q, k_pages, v_pages)
     dp = decode_head_dim(head_dim, cdt)
@@ -325,7 +324,7 @@ def write_to_paged_cache_rope(
                                     sections, seq_lens)
     if q_rot is not None:
         return q_rot, k_pages, v_pages
-    from .cache import _check_positions, _positions
+    from .cache import _check_positions
     from .rope_axes import (check_axis_positions, check_sections, check_tables, device_positions, rows_of, sections4,
                             strides3)
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
@@ -367,10 +366,11 @@ def write_to_paged_cache_rope(
     if q_rot.numel() == 0:
         return q_rot, k_pages, v_pages
     q, k, v = (rows_of(t.detach()) for t in (q, k, v))
-    table = table.to(device=dev, dtype=torch.int32).contiguous()
-    pos, stride = _positions(position, batch, dev)
+    table = _lib.device_ints(table, dev)
+    pos, stride = _check_positions(position, batch)
+    pos = _lib.device_ints(pos, dev)
     if seq_lens is not None:
-        seq_lens = seq_lens.to(device=dev, dtype=torch.int32).contiguous()
+        seq_lens = _lib.device_ints(seq_lens, dev)
     rope, rope_stride, i64 = None, (0, 0, 0), 0
     if rope_positions is not None:
         rope, rope_stride, i64 = device_positions(rope_positions, dev)
