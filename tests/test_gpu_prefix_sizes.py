@@ -143,3 +143,13 @@ def test_rotation_in_place_through_the_c_entry(dt, seq):
                              3, seq, 128, 0, _lib.dtype_tag(q))
     assert _lib.lib().pf_rope_axes(args, _lib.stream_of(q)) == _lib.PF_OK
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_no_prefix_and_no_sequences_as_lists():
+    q, k, v, _, _, table, lens = make("f32", 2, 4, 2, 64, 16, 0, [3, 30])
+    want = check((q, k, v, table[0, :0], 0, table, lens), "f32")
+    assert torch.equal(want, paged_flash_attention_prefix(q, k, v, [], 0, table, lens))
+    pre = table[0, :1]
+    want = check((q, k, v, pre, 3, table[:, :0], lens * 0), "f32")
+    assert torch.equal(want, paged_flash_attention_prefix(q, k, v, pre, 3, [[], []], lens * 0))
+    assert paged_flash_attention_prefix(q[:0], k, v, pre, 3, table[:0], []).shape == (0, 4, 1, 64)

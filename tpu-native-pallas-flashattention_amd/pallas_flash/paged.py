@@ -169,7 +169,8 @@ def paged_flash_attention_prefix(
     if tuple(context_lens.shape) != (batch,):
         raise ValueError(f"context_lens must be [batch], got {tuple(context_lens.shape)}")
     for name, t in (("prefix_table", prefix_table), ("block_tables", block_tables), ("context_lens", context_lens)):
-        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        # (an empty list makes a float tensor)
+        if t.numel() > 0 and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool):
             raise ValueError(f"{name} must hold integers, got {t.dtype}")
     reach = prefix_table.shape[0] * page_size
     on_device = isinstance(prefix_len, torch.Tensor) and prefix_len.device.type != "cpu"
