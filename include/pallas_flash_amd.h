@@ -339,7 +339,8 @@ int pf_paged_attn_noalloc(const pf_paged_attn_args* args, void* stream);
  * workspace: at least pf_paged_prefix_attn_workspace_size(args) bytes, 256-byte
  * aligned device memory (contents on entry do not matter). The size depends on
  * the shapes and prefix_len, not on pointers or what the device holds; 0: the
- * call would be refused.
+ * call would be refused. More than 2^31 - 2^20 prefix, own or query rows, or
+ * 2^24 workgroups (about: batch * num_kv_heads): PF_ERR_UNSUPPORTED.
  * ------------------------------------------------------------------------- */
 typedef struct {
   const void* q;

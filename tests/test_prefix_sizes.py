@@ -40,3 +40,13 @@ def test_lengths_past_the_range_are_refused(L):
     shape = dict(batch=128, num_heads=256, num_kv_heads=1, dtype=1)
     assert L.pf_paged_prefix_attn_workspace_size(long_prefix(MOST + 1, **shape)) == 0
     assert L.pf_paged_prefix_attn(long_prefix(MOST + 1, **shape), None) == _lib.PF_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("batch,heads", [(600_000, 32), (1 << 24, 1)])
+def test_batches_past_the_launch_are_refused(L, batch, heads):
+    """A launch has fewer than 2^32 threads: the merge's 256 for each sequence and KV head, at least."""
+    a = dict(batch=batch, num_heads=heads, num_kv_heads=heads, dtype=1)
+    assert L.pf_paged_prefix_attn_workspace_size(long_prefix(2048, **a)) == 0
+    assert L.pf_paged_prefix_attn(long_prefix(2048, **a), None) == _lib.PF_ERR_UNSUPPORTED
+    a["batch"] = (1 << 24) // heads - 1
+    assert L.pf_paged_prefix_attn_workspace_size(long_prefix(2048, **a)) > 0

@@ -1002,7 +1002,10 @@ int fill_prefix(const pf_paged_prefix_attn_args* a, pf::PrefixParams* p, int* D)
   p->thin = p->dma && p->g <= 16 && (p->dma > 1 || a->page_size % std::max(4, rows_per_load) == 0) &&
             ((uintptr_t)a->q & 15) == 0;
   const int64_t n_pre = a->batch > 0 ? plan_prefix(p, *D, es) : 0;
-  if (n_pre + p->own.n_waves > kMaxGrid) return PF_ERR_UNSUPPORTED;
+  // A launch has fewer than 2^32 threads: workgroups of 256.
+  constexpr int64_t kMostWgs = ((int64_t)1 << 24) - 1;
+  const int64_t merge = a->batch > 0 ? (int64_t)a->batch * p->Hkv * ((p->g + p->merge_heads - 1) / p->merge_heads) : 0;
+  if (n_pre + p->own.n_waves > kMostWgs || merge > kMostWgs) return PF_ERR_UNSUPPORTED;
   p->n_pre = (int)n_pre;
   return PF_OK;
 }
