@@ -153,3 +153,36 @@ def test_no_prefix_and_no_sequences_as_lists():
     want = check((q, k, v, pre, 3, table[:, :0], lens * 0), "f32")
     assert torch.equal(want, paged_flash_attention_prefix(q, k, v, pre, 3, [[], []], lens * 0))
     assert paged_flash_attention_prefix(q[:0], k, v, pre, 3, table[:0], []).shape == (0, 4, 1, 64)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_rotation_with_its_gradient_captured(dt):
+    """Forward and backward in one graph, replayed with new positions, inputs and gradients between eager steps."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    new = lambda h: torch.randn(2, 33, h, 64, device="cuda", generator=gen).to(dt).transpose(1, 2)  # noqa: E731
+    cos, sin = precompute_rope(200, 64, 10000.0, device="cuda")
+    pos = torch.zeros(3, 2, 33, dtype=torch.int64, device="cuda")
+    x, y, gx, gy = new(6), new(2), new(6), new(2)
+
+    def step():
+        q, k = (t.detach().requires_grad_() for t in (x, y))
+        out = apply_rope_axes(q, k, pos, cos, sin, (8, 12, 12))
+        return [*(t.detach() for t in out), *torch.autograd.grad(out, (q, k), (gx, gy))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        pos.random_(-1, 201, generator=gen)
+        for t in (x, y, gx, gy):
+            t.copy_(new(t.shape[1]))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
