@@ -330,7 +330,8 @@ int pf_paged_attn_noalloc(const pf_paged_attn_args* args, void* stream);
  *     not be full
  *   prefix_len_ptr: device int32 or NULL; given, the prefix has
  *     max(0, min(*prefix_len_ptr, prefix_len)) keys (a captured call can follow
- *     a prefix that grows)
+ *     a prefix that grows). The work is divided for prefix_len keys: the nearer
+ *     it is to what the prefix will have, the faster
  *   block_tables [batch, pages_per_seq], context_lens [batch] int32 (device):
  *     the sequences' own pages and keys, the prefix not counted
  * Sequence b attends prefix + min(context_lens[b], pages_per_seq * page_size)

@@ -336,7 +336,7 @@ int decode_stream_waves(int dtype, int head_dim, int stages, int group, bool fin
 int decode_stream_qrows(int group);               // query rows per partial slot
 hipError_t launch_decode_stream(const DecodeParams& p, int dtype, bool paged, hipStream_t stream);
 
-// Attention of a batch over a shared prefix (attn_prefix.hip).
+// Attention of a batch over a shared prefix (attn_prefix.hpp).
 constexpr int kPrefixRows = 128;  // query rows per workgroup
 constexpr int kMergeLoads = 8;    // partials in flight per lane of the merge
 // Chunks of `chunk` keys that hold len keys. (len + chunk may pass 2^31; every

@@ -127,7 +127,9 @@ def paged_flash_attention_prefix(
     its own. The result is that of ``paged_flash_attention`` with the prefix's
     tokens ahead of every sequence's; the prefix's K/V are read once for the
     batch instead of once per sequence (the reference's paged call,
-    paged.py:102-192, knows no sharing).
+    paged.py:102-192, knows no sharing). Two launches: where the prefix is short
+    and the sequences few, ``paged_flash_attention`` over joined tables can be
+    faster (5 us for 9).
 
     Args:
         q: ``[batch, num_heads, 1, head_dim]``.
@@ -136,7 +138,10 @@ def paged_flash_attention_prefix(
         prefix_len: tokens of the prefix: an int in ``[0, prefix_pages *
             page_size]`` (its last page need not be full), or a one-entry
             integer tensor on the device, which is not read back (the call stays
-            capturable) and counts up to the table's reach.
+            capturable) and counts up to the table's reach. The work is divided
+            for that reach: a prefix that fills little of a long table takes
+            longer than with its length on the host (1000 tokens of 65536: 28 us
+            for 15; of 2000: 15), so give a table near what it will hold.
         block_tables, context_lens: the sequences' own pages and tokens as
             ``paged_flash_attention`` takes them, the prefix not counted. A
             sequence without tokens at all yields zeros.
